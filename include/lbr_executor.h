@@ -31,6 +31,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "lbr_paged.h"   /* the op codes that the reference does not have */
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -175,6 +177,15 @@ int lbr_plan_launch(lbr_plan* plan);
 
 /* Wait for all work on the library stream. */
 int lbr_synchronize(void);
+
+/* Order the library stream with a stream of the caller's (a hipStream_t of
+ * the same device; NULL: the legacy default stream), for device memory that
+ * both touch: lbr_wait_stream holds later launches back until what `stream`
+ * has been given so far is done, lbr_signal_stream holds later work of
+ * `stream` back until the launches so far are done.  Neither waits on the
+ * host. */
+int lbr_wait_stream(void* stream);
+int lbr_signal_stream(void* stream);
 
 /* Time `iters` back-to-back lbr_plan_launch calls with hipEvents recorded
  * on the library stream; *out_ms = total elapsed milliseconds. */

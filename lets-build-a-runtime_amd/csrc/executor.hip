@@ -239,6 +239,14 @@ static decode_fn decoder_for(int op) {
             return decode_attention;
         case OP_GATED_ACT:
             return decode_gated_act;
+        case OP_CACHE_WRITE:
+            return decode_cache_write;
+        case OP_CACHE_READ:
+            return decode_cache_read;
+        case OP_PAGED_ATTENTION:
+            return decode_paged_attention;
+        case OP_VERIFY_DRAFT:
+            return decode_verify_draft;
         default:
             return nullptr;  // OP_PERMUTE has no kernel, as in the reference
     }
@@ -876,6 +884,26 @@ int lbr_memset(void* dst, int value, size_t bytes) {
     HIP_TRY(hipMemsetAsync(dst, value, bytes, g_stream));
     HIP_TRY(hipStreamSynchronize(g_stream));
     return LBR_OK;
+}
+
+static int order_streams(hipStream_t first, hipStream_t second) {
+    hipEvent_t e;
+    HIP_TRY(hipEventCreateWithFlags(&e, hipEventDisableTiming));
+    hipError_t rc = hipEventRecord(e, first);
+    if (rc == hipSuccess) rc = hipStreamWaitEvent(second, e, 0);
+    (void)hipEventDestroy(e);   // released once the recorded work has passed it
+    HIP_TRY(rc);
+    return LBR_OK;
+}
+
+int lbr_wait_stream(void* stream) {
+    int rc = ensure_init();
+    return rc ? rc : order_streams((hipStream_t)stream, g_stream);
+}
+
+int lbr_signal_stream(void* stream) {
+    int rc = ensure_init();
+    return rc ? rc : order_streams(g_stream, (hipStream_t)stream);
 }
 
 int lbr_execute(const OpNode* nodes, int n_nodes) {

@@ -432,6 +432,11 @@ Rng input_rng(const OpNode* nd, int k) {
             e = k == 0 ? mul({bh, S, hd}) : k <= 2 ? mul({kvh, S, hd}) : (k == 3 && x[3]) ? mul({bh, S, S}) : -1;
             break;
         }
+        case OP_CACHE_WRITE: case OP_CACHE_READ: case OP_PAGED_ATTENTION: case OP_VERIFY_DRAFT: {
+            const long long b = lbr_paged_input_bytes(nd, k);
+            if (b >= 0) return {p, p + (uintptr_t)b};
+            break;
+        }
         default:
             break;
     }

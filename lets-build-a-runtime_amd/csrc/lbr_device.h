@@ -428,6 +428,12 @@ bool lbr_tuned_fp32_size(long long M, long long N, long long K);
 int gemm_dma_tile_by_name(const Step& s, const char* name);
 int gemm_dma_written(const Step& s, void** ptr, size_t* bytes, int cap);
 int decode_attention(const OpNode* n, Step* s);
+int decode_cache_write(const OpNode* n, Step* s);
+int decode_cache_read(const OpNode* n, Step* s);
+int decode_paged_attention(const OpNode* n, Step* s);
+int decode_verify_draft(const OpNode* n, Step* s);
+// Bytes input k of a paged-cache or VERIFY_DRAFT node reads, -1 where its fields fix none.
+long long lbr_paged_input_bytes(const OpNode* n, int k);
 // Whether a decoded attention step can defer its store (its rows staged, then
 // written by a second kernel after every read of Q, K and V, so that O may lie
 // over them): the key-range split (merge kernel), the key-quartered kernel and

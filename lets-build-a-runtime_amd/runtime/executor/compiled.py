@@ -12,7 +12,11 @@ node filtering and OpNode contents.  What changes is where memory lives:
 * each graph input gets a fixed device staging buffer, so node pointers
   never change after compile and the launch sequence can be captured into a
   hipGraph once and replayed (``run`` = H2D inputs, graph launch, D2H
-  outputs).
+  outputs);
+* states (``Graph.states``: a key/value cache) have device memory of their own
+  that keeps its contents from run to run;
+* inputs and states can lie in the caller's device memory instead
+  (``device_tensors``: any object with ``__cuda_array_interface__``).
 
 ``launch()`` / ``synchronize()`` / ``time_launches()`` / ``profile_nodes()``
 run the plan on device-resident data for benchmarking.  There is no CPU
@@ -27,7 +31,7 @@ import time
 
 import numpy as np
 
-from ..ir import Graph, OpType
+from ..ir import STATE_WRITERS, Graph, OpType
 from ..planner import MemoryPlan
 from .common import Executor, OpTiming, RunProfile
 from .hip_lib import FUSE_KINDS, HipLibrary, live_arrays, load_library
@@ -77,6 +81,94 @@ class DeviceWeights:
         if self.base:
             self._lib.free(self.base)
             self.base = 0
+
+
+class DeviceStates:
+    """Device memory of a graph's states, by name; lent from one plan of a session to the next.
+    A state starts as zeros, or as its tensor's buffer."""
+
+    def __init__(self, lib: HipLibrary) -> None:
+        self._lib = lib
+        self._held: dict[str, tuple[int, int]] = {}            # name -> (device ptr, bytes)
+        self._bound: dict[str, tuple[int, int, object]] = {}   # the same in the caller's memory, its tensor
+
+    def take(self, graph: Graph, name: str) -> int:
+        """Device address of state `name`, allocated and initialised on its first use."""
+        t = graph.tensors[name]
+        nb = int(np.prod(t.shape)) * np.dtype(t.dtype).itemsize
+        ptr, have = (self._bound.get(name) or self._held.get(name) or (0, nb))[:2]
+        if have != nb:
+            raise ValueError(f"state '{name}' holds {have} bytes, graph expects {nb}")
+        if ptr:
+            return ptr
+        ptr = self._lib.alloc(nb)
+        self._held[name] = (ptr, nb)
+        if t.buffer is not None and nb:
+            buf = np.ascontiguousarray(t.buffer)
+            self._lib.h2d(ptr, buf.ctypes.data, nb)
+        elif nb:
+            self._lib.check(self._lib.lbr_memset(ctypes.c_void_p(ptr), 0, nb), "state clear")
+        return ptr
+
+    def bind(self, name: str, ptr: int, nbytes: int, tensor) -> None:
+        """Put a state into the caller's memory, before any plan uses it."""
+        have = self._bound.get(name) or self._held.get(name)
+        if have is not None and have[0] != ptr:
+            raise ValueError(f"state '{name}' has its memory already; plans use it")
+        self._bound[name] = (ptr, nbytes, tensor)
+
+    def range(self, name: str) -> tuple[int, int]:
+        """(device address, bytes) of a state that a plan uses."""
+        if name not in self._bound and name not in self._held:
+            raise KeyError(f"no state '{name}'")
+        return (self._bound.get(name) or self._held[name])[:2]
+
+    def free(self) -> None:
+        for ptr, _ in self._held.values():
+            self._lib.free(ptr)
+        self._held, self._bound = {}, {}
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class DeviceArray:
+    """A plan's device buffer for other libraries to look at without a copy
+    (``torch.as_tensor(array, device="cuda")``); it keeps the executor alive.  The library's stream
+    writes it: synchronise, or order another stream behind it with ``signal_stream``, before a read."""
+
+    def __init__(self, owner: "CompiledExecutor", address: int, shape: tuple[int, ...], dtype: str) -> None:
+        self.owner = owner
+        self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": np.dtype(dtype).str,
+                                         "data": (address, False), "version": 2}
+
+
+def _device_range(obj, name: str, shape: tuple[int, ...], dtype: str, device: int) -> int:
+    """Device address of the caller's tensor for graph tensor `name`, checked against it."""
+    face = getattr(obj, "__cuda_array_interface__", None)
+    if face is None:
+        raise TypeError(f"device tensor '{name}': {type(obj).__name__} is not in device memory "
+                        f"(no __cuda_array_interface__)")
+    at = getattr(getattr(obj, "device", None), "index", None)
+    if at is not None and at != device:
+        raise ValueError(f"device tensor '{name}' is on device {at}, the executor on {device}")
+    if tuple(face["shape"]) != tuple(shape):
+        raise ValueError(f"device tensor '{name}' has shape {tuple(face['shape'])}, graph expects {tuple(shape)}")
+    have = np.dtype(face["typestr"])
+    if have != np.dtype(dtype):
+        raise ValueError(f"device tensor '{name}' is {have}, graph expects {dtype}")
+    step = have.itemsize
+    for d, s in zip(reversed(face["shape"]), reversed(face.get("strides") or ())):
+        if d > 1 and s != step:
+            raise ValueError(f"device tensor '{name}' is not contiguous")
+        step *= max(d, 1)
+    ptr = int(face["data"][0] or 0)
+    if ptr % 16:
+        raise ValueError(f"device tensor '{name}' does not start on a 16-byte boundary")
+    return ptr
 
 
 class _PinnedBlock:
@@ -147,7 +239,8 @@ class CompiledExecutor(Executor):
     """Plan → device OpNode array → hipGraph, replayed per run()."""
 
     def __init__(self, profile: bool = False, use_graph: bool = True, device: int = 0,
-                 weights: DeviceWeights | None = None, fuse: bool | None = None) -> None:
+                 weights: DeviceWeights | None = None, fuse: bool | None = None,
+                 states: DeviceStates | None = None, device_tensors: dict | None = None) -> None:
         super().__init__(profile=profile)
         self._use_graph = use_graph
         # peephole fusion in the device library (LBR_FUSE=0 turns it off)
@@ -163,6 +256,11 @@ class CompiledExecutor(Executor):
         # graph's constants, never freed here; weights this executor uploads itself it owns
         self._weights: DeviceWeights | None = weights
         self._owns_weights = weights is None
+        # states passed in are the session's; without them this executor has its own
+        self._states: DeviceStates | None = states
+        self._owns_states = states is None
+        # the caller's tensors that graph inputs and states lie in (kept alive with the plan)
+        self._device_tensors = dict(device_tensors or {})
         self._inputs: dict[str, tuple[int, int]] = {}   # name -> (device ptr, nbytes)
         self._addr: dict[str, int] = {}
         self._pinned: PinnedPool | None = None
@@ -174,7 +272,7 @@ class CompiledExecutor(Executor):
         self._lib = lib
         graph = plan.graph
         self._graph = graph
-        external = set(graph.inputs) | set(graph.constants)
+        external = graph.external
 
         # constants referenced by dispatched nodes (and constant outputs)
         order = dispatch_order(plan)
@@ -200,9 +298,27 @@ class CompiledExecutor(Executor):
             self._weights = DeviceWeights(lib, graph, used_consts)
             self._owns_weights = True
 
+        bound: dict[str, int] = {}
+        for name, obj in self._device_tensors.items():
+            if name not in graph.inputs and name not in graph.states:
+                raise ValueError(f"device tensor '{name}' is neither an input nor a state of the graph")
+            t = graph.tensors[name]
+            bound[name] = _device_range(obj, name, t.shape, t.dtype, self._device)
+        if self._states is None:
+            self._states = DeviceStates(lib)
+        state_addr = {}
+        for name in graph.states:
+            if name in bound:
+                t = graph.tensors[name]
+                self._states.bind(name, bound[name], int(np.prod(t.shape)) * np.dtype(t.dtype).itemsize,
+                                  self._device_tensors[name])
+            state_addr[name] = self._states.take(graph, name)
+
         self._arena = lib.alloc(max(plan.arena_size, 1))
         self._inputs = {}
         for name in graph.inputs:
+            if name in bound:
+                continue
             t = graph.tensors[name]
             nb = int(np.prod(t.shape)) * np.dtype(t.dtype).itemsize
             self._inputs[name] = (lib.alloc(max(nb, 1)), nb)
@@ -215,6 +331,11 @@ class CompiledExecutor(Executor):
             addr[name] = ptr
         for name in used_consts:
             addr[name] = self._weights.addr(name)
+        addr.update({n: p for n, p in bound.items() if n in graph.inputs})
+        addr.update(state_addr)
+        for node in order:
+            if node.op in STATE_WRITERS:   # its output is the state itself
+                addr[node.output] = state_addr[graph.state_of(node.inputs[0])]
         self._addr = addr
 
         def resolve(name: str) -> int:
@@ -306,6 +427,9 @@ class CompiledExecutor(Executor):
         """Enqueue the input copies on the library stream (through its pinned ring); the
         caller's arrays may change once this returns."""
         graph = self._graph
+        for name in self._device_tensors:
+            if name in inputs:
+                raise ValueError(f"input '{name}' lies in the caller's device memory: write it there")
         for name, (ptr, nb) in self._inputs.items():
             if name not in inputs:
                 raise ValueError(f"Missing input tensor: '{name}'")
@@ -407,6 +531,41 @@ class CompiledExecutor(Executor):
     def device_address(self, name: str) -> int:
         return self._addr[name]
 
+    def device_outputs(self) -> dict[str, DeviceArray]:
+        """The graph outputs' device buffers; each launch writes them anew."""
+        g = self._graph
+        return {n: DeviceArray(self, self._addr[n], g.tensors[n].shape, g.tensors[n].dtype) for n in g.outputs}
+
+    def wait_stream(self, stream) -> None:
+        """Order later launches behind what `stream` (a torch stream or a hipStream_t) holds now."""
+        self._lib.check(self._lib.lbr_wait_stream(ctypes.c_void_p(getattr(stream, "cuda_stream", stream))),
+                        "lbr_wait_stream")
+
+    def signal_stream(self, stream) -> None:
+        """Order later work of `stream` behind the launches so far."""
+        self._lib.check(self._lib.lbr_signal_stream(ctypes.c_void_p(getattr(stream, "cuda_stream", stream))),
+                        "lbr_signal_stream")
+
+    # ------------------------------------------------------------------ states
+    def read_state(self, name: str) -> np.ndarray:
+        """A host copy of a state."""
+        ptr, nb = self._states.range(name)
+        t = self._graph.tensors[name]
+        out = np.empty(t.shape, dtype=t.dtype)
+        if nb:
+            self._lib.d2h(out.ctypes.data, ptr, nb)
+        return out
+
+    def write_state(self, name: str, value: np.ndarray) -> None:
+        """Replace a state's contents."""
+        ptr, nb = self._states.range(name)
+        t = self._graph.tensors[name]
+        arr = np.ascontiguousarray(value)
+        if arr.dtype != np.dtype(t.dtype) or arr.shape != tuple(t.shape):
+            raise ValueError(f"state '{name}' is {t.dtype} {tuple(t.shape)}, got {arr.dtype} {arr.shape}")
+        if nb:
+            self._lib.h2d(ptr, arr.ctypes.data, nb)
+
     # ------------------------------------------------------------------ teardown
     def close(self) -> None:
         lib = self._lib
@@ -427,6 +586,9 @@ class CompiledExecutor(Executor):
         if self._weights is not None and self._owns_weights:
             self._weights.free()
             self._weights = None
+        if self._states is not None and self._owns_states:
+            self._states.free()
+            self._states = None
 
     def release_weights(self) -> DeviceWeights | None:
         """Hand the resident weights to the caller (Session, which shares them between cached

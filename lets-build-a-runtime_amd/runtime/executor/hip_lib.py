@@ -72,6 +72,8 @@ class HipLibrary:
             "lbr_plan_num_nodes": ([c_vp], c_int),
             "lbr_plan_launch": ([c_vp], c_int),
             "lbr_synchronize": ([], c_int),
+            "lbr_wait_stream": ([c_vp], c_int),
+            "lbr_signal_stream": ([c_vp], c_int),
             "lbr_plan_time": ([c_vp, c_int, P(ctypes.c_float)], c_int),
             "lbr_plan_profile": ([c_vp, c_int, P(ctypes.c_float), c_int], c_int),
             "lbr_plan_node_kernel": ([c_vp, c_int, ctypes.c_char_p, c_int], c_int),

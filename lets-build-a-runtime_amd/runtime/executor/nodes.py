@@ -21,6 +21,7 @@ from typing import Callable
 
 import numpy as np
 
+from .. import paged
 from ..ir import FOLD_ONLY_BASE, Graph, Node, OpType
 from ..ops import OP_REGISTRY
 from ..planner import MemoryPlan
@@ -35,7 +36,7 @@ def is_dispatch_alias(node: Node) -> bool:
 def dispatch_order(plan: MemoryPlan) -> list[Node]:
     """Nodes that reach the executor, in plan order (compiled.py:50-60)."""
     graph = plan.graph
-    external = set(graph.inputs) | set(graph.constants)
+    external = graph.external
     out = []
     for node in plan.order:
         if is_dispatch_alias(node) and node.inputs[0] not in external:
@@ -194,6 +195,15 @@ def required_elements(node: Node, graph: Graph) -> list[tuple[str, int]]:
         if has_mask:
             need.append((ins[3], bh * S * S))
         return need
+    if op.name in paged.INPUTS:
+        # exact shapes and dtypes: what these kernels read is bounded by them and, for pages and
+        # positions, by the kernels' own checks
+        graph_ins = [graph.tensors[t] for t in ins]
+        paged.check_op(op.name, [t.shape for t in graph_ins], [t.dtype for t in graph_ins], node.attrs, out_shape,
+                       graph.tensors[node.output].dtype)
+        if op == OpType.CACHE_WRITE and graph.state_of(ins[0]) is None:
+            raise ValueError(f"CACHE_WRITE node {node.id} writes '{ins[0]}', which is not a state of the graph")
+        return [(t, _numel(graph.tensors[t].shape)) for t in ins]
     return []
 
 
@@ -206,5 +216,6 @@ def check_extents(order: list[Node], graph: Graph) -> None:
             if need > have:
                 raise ValueError(f"node {node.id} ({node.op.name}) would read {need} elements of '{name}', "
                                  f"which holds {have}")
-        if node.op not in (OpType.RESHAPE, OpType.TRANSPOSE, OpType.SLICE, OpType.CAT) and out_dtype != "float32":
+        if (node.op not in (OpType.RESHAPE, OpType.TRANSPOSE, OpType.SLICE, OpType.CAT)
+                and node.op.name not in paged.INPUTS and out_dtype != "float32"):
             raise ValueError(f"node {node.id} ({node.op.name}) produces {out_dtype}; device kernels compute fp32")

@@ -32,8 +32,10 @@ class OpType(Enum):
     """Operator codes (value = the C ABI op code).
 
     Ranges: 100-199 unary, 200-299 binary, 300-399 reductions, 400-499
-    matmul, 500-599 data movement, 600-699 normalisation, 1000-1499 fused,
-    5000+ fold-only (evaluated by constant folding, never dispatched).
+    matmul, 500-599 data movement, 600-699 normalisation, 1000-1499 fused
+    (1100-1199: the paged key/value cache and drafted tokens, which the
+    reference has no counterpart of), 5000+ fold-only (evaluated by constant
+    folding, never dispatched).
     """
     RELU = 100
     EXP = 101
@@ -72,6 +74,12 @@ class OpType(Enum):
     ATTENTION = 1002     # inputs [Q, K, V(, mask)], attrs["causal", "group_size"]
     GATED_ACT = 1003     # inputs [x, up] / [x, bias, up], attrs["act", "has_bias"]
 
+    # attrs of the cache ops: "page_size", "kv_heads", "head_dim", "cache_type" (runtime/paged.py)
+    CACHE_WRITE = 1100       # inputs [cache, K, V, page_table, start, count]; output: the cache itself
+    CACHE_READ = 1101        # inputs [cache, page_table, start, count], attrs["length"]
+    PAGED_ATTENTION = 1102   # inputs [Q, cache, page_table, start, count], attrs["scale"]
+    VERIFY_DRAFT = 1103      # inputs [target, draft, tokens, uniforms, count]
+
     CAST = 5000
     EXPAND = 5001
     ARANGE = 5002
@@ -86,6 +94,9 @@ class OpType(Enum):
 
 # Op codes at or above this value are fold-only.
 FOLD_ONLY_BASE = 5000
+
+# Ops whose output is their first input's own memory, a state they write in place.
+STATE_WRITERS = frozenset({OpType.CACHE_WRITE})
 
 
 @dataclass
@@ -120,6 +131,9 @@ class Graph:
         self.inputs: list[str] = []
         self.outputs: list[str] = []
         self.constants: list[str] = []
+        # tensors that stay on the device from run to run (a key/value cache): neither fed nor
+        # folded, zero at first unless they have a buffer, changed by the STATE_WRITERS alone
+        self.states: list[str] = []
         self._producer: dict[str, int] = {}
         self._consumers: dict[str, list[int]] = {}
         # symbol -> [(input tensor name, dim index)], set by the exporter
@@ -134,6 +148,12 @@ class Graph:
         info = TensorInfo(name=name, shape=shape, dtype=dtype)
         self.tensors[name] = info
         self._consumers[name] = []
+        return info
+
+    def add_state(self, name: str, shape: tuple[int, ...], dtype: str = "uint8") -> TensorInfo:
+        """A tensor that the executor keeps on the device between runs."""
+        info = self.add_tensor(name, shape, dtype)
+        self.states.append(name)
         return info
 
     def add_node(self, op: OpType, inputs: list[str], output: str,
@@ -159,6 +179,22 @@ class Graph:
 
     def consumers(self, tensor_name: str) -> list[Node]:
         return [self.nodes[i] for i in self._consumers.get(tensor_name, [])]
+
+    @property
+    def external(self) -> set[str]:
+        """Tensors with memory of their own outside the arena: inputs, constants, states, and
+        the outputs of state writers, which are those states."""
+        written = {n.output for n in self.nodes.values() if n.op in STATE_WRITERS}
+        return set(self.inputs) | set(self.constants) | set(self.states) | written
+
+    def state_of(self, tensor_name: str) -> str | None:
+        """The state whose memory the tensor is: itself, or the one its writer was given."""
+        while tensor_name not in self.states:
+            node = self.producer(tensor_name)
+            if node is None or node.op not in STATE_WRITERS:
+                return None
+            tensor_name = node.inputs[0]
+        return tensor_name
 
     # ------------------------------------------------------------ ordering
     def _toposort(self) -> list[Node]:
@@ -214,7 +250,7 @@ class Graph:
     # ------------------------------------------------------------ serialisation
     def to_dict(self) -> dict:
         """Structure only (no weight data); nodes in topological order."""
-        return {
+        d = {
             "nodes": [{"id": n.id, "op": n.op.name, "inputs": n.inputs, "output": n.output, "attrs": n.attrs}
                       for n in self._toposort()],
             "tensors": {name: {"shape": list(t.shape), "dtype": t.dtype} for name, t in self.tensors.items()},
@@ -222,6 +258,9 @@ class Graph:
             "constants": self.constants,
             "outputs": self.outputs,
         }
+        if self.states:   # graphs without states keep the reference's format
+            d["states"] = self.states
+        return d
 
     @classmethod
     def from_dict(cls, d: dict) -> "Graph":
@@ -231,6 +270,7 @@ class Graph:
         g.inputs = d["inputs"]
         g.constants = d["constants"]
         g.outputs = d["outputs"]
+        g.states = d.get("states", [])
         for nd in d["nodes"]:
             g.add_node(OpType[nd["op"]], nd["inputs"], nd["output"], nd.get("attrs"))
         return g

@@ -22,6 +22,7 @@ from typing import Any, Callable
 
 import numpy as np
 
+from . import paged
 from .ir import Graph, Node, OpType
 
 NumpyEvaluator = Callable[[list[np.ndarray], dict[str, Any]], np.ndarray]
@@ -280,6 +281,20 @@ def _slice_extras(node: Node, graph: Graph) -> list[int]:
     return [outer, shape[dim], start, end - start, inner]
 
 
+def _paged_extras(node: Node, graph: Graph) -> list[int]:
+    """runtime/paged.py:op_extras; PAGED_ATTENTION appends the bits of its score scale."""
+    ex = paged.op_extras(node.op.name, [graph.tensors[t].shape for t in node.inputs], node.attrs)
+    if node.op == OpType.PAGED_ATTENTION:
+        scale = node.attrs.get("scale")
+        ex.append(_float_bits(1.0 / np.sqrt(node.attrs["head_dim"]) if scale is None else scale))
+    return ex
+
+
+def _verify_extras(node: Node, graph: Graph) -> list[int]:
+    """[vocabulary]"""
+    return [graph.tensors[node.inputs[0]].shape[-1]]
+
+
 # ---------------------------------------------------------------- shape rules
 
 def _shape_broadcast_binary(in_shapes, attrs):
@@ -352,6 +367,14 @@ def _shape_cat(in_shapes, attrs):
     s = list(in_shapes[0])
     s[dim] = sum(x[dim] for x in in_shapes)
     return tuple(s)
+
+
+def _shape_cache_read(in_shapes, attrs):
+    return (2, in_shapes[1][0], attrs["kv_heads"], attrs["length"], attrs["head_dim"])
+
+
+def _shape_verify(in_shapes, attrs):
+    return (in_shapes[2][0], in_shapes[2][1] + 1)
 
 
 # ---------------------------------------------------------------- scratch
@@ -429,6 +452,13 @@ OP_REGISTRY: dict[OpType, OpDef] = {
                             evaluator=_eval_attention),
     OpType.GATED_ACT: OpDef(extras=_gated_act_extras, evaluator=_eval_gated_act),
 
+    # the paged cache and drafted tokens (runtime/paged.py); no numpy evaluators: their inputs are
+    # states and per-call tensors, never all constant
+    OpType.CACHE_WRITE: OpDef(extras=_paged_extras),
+    OpType.CACHE_READ: OpDef(extras=_paged_extras, shape=_shape_cache_read),
+    OpType.PAGED_ATTENTION: OpDef(extras=_paged_extras),
+    OpType.VERIFY_DRAFT: OpDef(extras=_verify_extras, shape=_shape_verify),
+
     # fold-only
     OpType.ARANGE: OpDef(evaluator=lambda ins, a: np.arange(a["start"], a["end"], dtype=np.dtype(a["dtype"])),
                          shape=lambda in_shapes, a: (a["end"] - a["start"],)),
@@ -473,6 +503,7 @@ def resolve_graph(graph: Graph, bindings: dict[str, int]) -> Graph:
     out.inputs = list(graph.inputs)
     out.outputs = list(graph.outputs)
     out.constants = list(graph.constants)
+    out.states = list(graph.states)
     out.dynamic_dims = graph.dynamic_dims
 
     new_shapes = {}

@@ -24,7 +24,7 @@ from typing import Callable
 
 import numpy as np
 
-from ..ir import Graph, Node, OpType
+from ..ir import STATE_WRITERS, Graph, Node, OpType
 from ..ops import OP_REGISTRY
 
 Pass = Callable[[Graph], bool]
@@ -237,7 +237,8 @@ def eliminate_dead_code(graph: Graph) -> bool:
     changed = False
     outs = set(graph.outputs)
     while True:
-        dead = [n for n in graph.nodes.values() if not graph.consumers(n.output) and n.output not in outs]
+        dead = [n for n in graph.nodes.values() if not graph.consumers(n.output) and n.output not in outs
+                and n.op not in STATE_WRITERS]   # a state written now is read by a later run
         if not dead:
             break
         for n in dead:

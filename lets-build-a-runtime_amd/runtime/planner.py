@@ -135,7 +135,7 @@ def _memory_aware_order(graph: Graph) -> list[Node]:
     for n in graph.nodes.values():
         for t in n.inputs:
             uses_left[t] += 1
-    external = set(graph.inputs) | set(graph.constants)
+    external = graph.external
 
     def freed(n: Node) -> int:
         return sum(_tensor_size(graph, t) for t in n.inputs if t not in external and uses_left[t] == 1)
@@ -198,7 +198,7 @@ def _resolve_alias(name: str, graph: Graph) -> str:
 def _compute_lifetimes(graph: Graph, order: list[Node],
                        config: PlannerConfig | None = None) -> tuple[dict[str, Lifetime], dict[str, str]]:
     config = config or PlannerConfig()
-    external = set(graph.inputs) | set(graph.constants)
+    external = graph.external
     memory_root: dict[str, str] = {}
 
     def root_of(name: str) -> str:
@@ -331,7 +331,7 @@ def plan(graph: Graph, config: PlannerConfig | None = None) -> MemoryPlan:
     offsets = {k: v for k, v in offsets_all.items() if k not in scratch_names}
     scratch = {nid: (offsets_all[n], size) for nid, (n, size) in scratch_info.items()}
 
-    external = set(graph.inputs) | set(graph.constants)
+    external = graph.external
     inter = [n for n in graph.tensors if n not in external]
     stats = PlanStats(
         arena_bytes=arena_size,

@@ -13,6 +13,13 @@ resident across ``rebind`` calls when the constants are unchanged.
 ``execution_mode="interpreted"`` (the reference's per-node CPU debug path)
 is not provided by this backend and raises.
 
+A graph's states (``Graph.states``: the key/value caches of a model that continues
+its sequences) stay on the device between runs, shared by every plan of the session;
+``read_state`` / ``write_state`` / ``reset_states`` move them.  ``device_tensors`` puts graph
+inputs and states into device memory the caller owns, and ``device_outputs`` shows the outputs
+there, for programs whose data never leaves the GPU (a program that shares memory with torch
+imports torch before its first session, so that both use the same HIP runtime).
+
 ``rebind`` keeps the last ``plan_cache`` compiled plans (arena, node array,
 hipGraph) keyed by their bindings: returning to a shape seen before switches
 to its plan without re-planning or re-capturing.  All cached plans share one
@@ -50,15 +57,19 @@ class Session:
         self._plan_cache = 8
         self._key = None
         self._weights: list = []      # device weight blocks shared by the cached executors
+        self._states = None           # device memory of the graph's states, shared by them too
 
     @staticmethod
-    def _bindings_key(bindings: dict[str, int] | None):
-        return tuple(sorted((bindings or {}).items()))
+    def _bindings_key(bindings: dict[str, int] | None, device_tensors: dict | None = None):
+        """The cache key of a plan: its symbols, and where its inputs lie if that is the caller's memory."""
+        at = tuple(sorted((n, _address(t)) for n, t in (device_tensors or {}).items()))
+        return tuple(sorted((bindings or {}).items())) + (("device_tensors", at) if at else ())
 
     @property
     def cached_plans(self) -> list:
         """Bindings of the compiled plans kept for rebind, least recently used first."""
-        return [dict(k) for k in self._plans]
+        return [dict(p for p in k if isinstance(p, tuple) and len(p) == 2 and isinstance(p[1], int))
+                for k in self._plans]
 
     @property
     def graph(self) -> Graph:
@@ -91,13 +102,16 @@ class Session:
     def create(self, execution_mode: str = "compiled", backend: str = "hip", optimization: str = "default",
                pipeline: list[Pass] | None = None, verbose: bool = False, profile: bool = False,
                bindings: dict[str, int] | None = None, validation: str = "normal",
-               use_graph: bool = True, plan_cache: int = 8) -> None:
+               use_graph: bool = True, plan_cache: int = 8, device_tensors: dict | None = None) -> None:
         """Optimise (once), resolve ``bindings``, plan, validate and compile.
 
         optimization: "none" | "default" (pipeline once) | "aggressive" (until stable)
         validation:   "strict" (fail on warnings) | "normal" (fail on errors) | "none"
         use_graph:    capture the launch sequence into a hipGraph (default) or launch eagerly
         plan_cache:   compiled plans kept for rebind (≥ 1)
+        device_tensors: name → tensor in device memory (``__cuda_array_interface__``, contiguous, on a
+                      16-byte boundary) that a graph input or state lies in from now on; the caller orders
+                      its own stream with the library's (``executor.wait_stream`` / ``signal_stream``)
         """
         self.close()
         self._execution_mode = execution_mode
@@ -140,15 +154,16 @@ class Session:
         self._validate(Phase.PRE_EXECUTE, ExecutionPlan(self._resolved, mem, execution_mode, backend), fail_on,
                        verbose)
 
-        ex = self._make_executor(execution_mode, backend, profile)
+        ex = self._make_executor(execution_mode, backend, profile, device_tensors=device_tensors)
         ex.compile(mem)
-        self._adopt(self._bindings_key(bindings), ex)
+        self._adopt(self._bindings_key(bindings, device_tensors), ex)
 
-    def rebind(self, bindings: dict[str, int]) -> None:
+    def rebind(self, bindings: dict[str, int], device_tensors: dict | None = None) -> None:
         """Switch to new symbol values (passes are not re-run): the cached plan for these
         bindings if there is one, else re-resolve, re-plan and re-compile (session.py:187-207
-        of the reference), sharing the resident weights."""
-        key = self._bindings_key(bindings)
+        of the reference), sharing the resident weights and the states.  ``device_tensors`` as in
+        ``create``; inputs they do not name have staging buffers again, states stay where they are."""
+        key = self._bindings_key(bindings, device_tensors)
         if key == self._key and self._executor is not None:
             return
         if key in self._plans:
@@ -162,7 +177,8 @@ class Session:
         self._memory_plan = mem
         self._plan_stats = mem.stats
         ex = self._make_executor(self._execution_mode, self._backend, self._profile,
-                                 weights=self._weights[-1] if self._weights else None)
+                                 weights=self._weights[-1] if self._weights else None,
+                                 device_tensors=device_tensors)
         ex.compile(mem)
         self._adopt(key, ex)
 
@@ -177,6 +193,31 @@ class Session:
             if profile:
                 self._executor._profile = self._profile
 
+    def device_outputs(self) -> dict:
+        """The current plan's output buffers on the device (``__cuda_array_interface__``): each
+        ``executor.launch()`` or ``run`` writes them anew."""
+        return self._ready().device_outputs()
+
+    def read_state(self, name: str) -> np.ndarray:
+        """A host copy of a state."""
+        return self._ready().read_state(name)
+
+    def write_state(self, name: str, value: np.ndarray) -> None:
+        """Replace a state's contents."""
+        self._ready().write_state(name, value)
+
+    def reset_states(self) -> None:
+        """Every state back to what it was at first: its tensor's buffer, or zeros."""
+        ex = self._ready()
+        for name in self._resolved.states:
+            t = self._resolved.tensors[name]
+            ex.write_state(name, np.zeros(t.shape, t.dtype) if t.buffer is None else t.buffer)
+
+    def _ready(self):
+        if self._executor is None:
+            raise RuntimeError("Session not created — call create() first")
+        return self._executor
+
     def close(self) -> None:
         """Free every cached plan's device memory and the weights now (otherwise freed when
         the session is collected)."""
@@ -190,6 +231,9 @@ class Session:
             w.free()
         self._plans.clear()
         self._weights = []
+        if self._states is not None:
+            self._states.free()
+        self._states = None
         self._executor = None
         self._key = None
 
@@ -227,10 +271,20 @@ class Session:
             for r in results:
                 print(r)
 
-    def _make_executor(self, execution_mode: str, backend: str, profile: bool = False, weights=None) -> Executor:
+    def _make_executor(self, execution_mode: str, backend: str, profile: bool = False, weights=None,
+                       device_tensors: dict | None = None) -> Executor:
         self._check_mode(execution_mode)
-        from .executor.compiled import CompiledExecutor
-        return CompiledExecutor(profile=profile, use_graph=getattr(self, "_use_graph", True), weights=weights)
+        from .executor.compiled import CompiledExecutor, DeviceStates
+        if self._graph.states and self._states is None:
+            from .executor.hip_lib import load_library
+            self._states = DeviceStates(load_library(0))
+        return CompiledExecutor(profile=profile, use_graph=getattr(self, "_use_graph", True), weights=weights,
+                                states=self._states, device_tensors=device_tensors)
+
+
+def _address(tensor) -> int:
+    face = getattr(tensor, "__cuda_array_interface__", None)
+    return int(face["data"][0] or 0) if face else 0
 
 
 def _validation_severity(validation: str) -> Severity | None:

@@ -2,9 +2,10 @@
 
 ``compiled_dispatch`` checks that every op the compiled executor will
 dispatch has a device kernel.  The set below is the device library's
-dispatch table (include/lbr_executor.h, lbr_op_supported); it equals the
+dispatch table (include/lbr_executor.h, lbr_op_supported): the
 reference's ``_C_DISPATCH_OPS`` (execution.py:16-34) — PERMUTE is the one
-registered op without a kernel on either side.
+registered op without a kernel on either side — and the ops of the paged
+cache and of drafted tokens, which the reference does not have.
 
 ``device_extents`` is specific to this backend: it refuses a plan in which
 a kernel would read past the end of an input (the reference's CPU code has
@@ -27,6 +28,7 @@ _HIP_DISPATCH_OPS: frozenset[OpType] = frozenset({
     OpType.RESHAPE, OpType.TRANSPOSE, OpType.SLICE, OpType.EMBEDDING, OpType.CAT,
     OpType.LAYERNORM, OpType.RMSNORM,
     OpType.MATMUL_ADD, OpType.FUSED_BIAS_RELU, OpType.ATTENTION, OpType.GATED_ACT,
+    OpType.CACHE_WRITE, OpType.CACHE_READ, OpType.PAGED_ATTENTION, OpType.VERIFY_DRAFT,
 })
 
 # name kept for callers written against the reference
@@ -35,7 +37,7 @@ _C_DISPATCH_OPS = _HIP_DISPATCH_OPS
 
 def _ops_needing_dispatch(plan: ExecutionPlan) -> list[tuple[int, OpType]]:
     graph = plan.graph
-    external = set(graph.inputs) | set(graph.constants)
+    external = graph.external
     out = []
     for node in plan.memory.order:
         op_def = OP_REGISTRY.get(node.op)

@@ -28,7 +28,7 @@ from __future__ import annotations
 from collections import defaultdict
 from numbers import Integral
 
-from ..ir import FOLD_ONLY_BASE, Graph, Node, OpType
+from ..ir import FOLD_ONLY_BASE, STATE_WRITERS, Graph, Node, OpType
 from ..ops import OP_REGISTRY
 from .core import Phase, Severity, ValidationResult, register_validator
 
@@ -94,8 +94,10 @@ def _structure(graph: Graph, validator: str) -> list[ValidationResult]:
     writers, readers = _writers_and_readers(graph)
     external = {t: "input" for t in graph.inputs}
     external.update({t: "constant" for t in graph.constants})
+    external.update({t: "state" for t in graph.states})
 
-    for role, names in (("input", graph.inputs), ("constant", graph.constants), ("output", graph.outputs)):
+    for role, names in (("input", graph.inputs), ("constant", graph.constants), ("state", graph.states),
+                        ("output", graph.outputs)):
         for t in names:
             if t not in table:
                 rep.error(f"graph {role} '{t}' is not in the tensor table")
@@ -123,13 +125,25 @@ def _structure(graph: Graph, validator: str) -> list[ValidationResult]:
             rep.error(f"{_who(nodes[0])} reads '{t}', which has no source: no node produces it and it is "
                       f"neither an input nor a constant")
 
+    # a state is written in place: each value of it, the state itself and every writer's output,
+    # has readers or one writer that goes on from it, and never both (a reader of the old value
+    # would have no order against the writer)
+    for t in table:
+        users = [n for n in readers.get(t, ()) if n.op in STATE_WRITERS and n.inputs and n.inputs[0] == t]
+        if users and graph.state_of(t) is None:
+            rep.error(f"{_who(users[0])} writes '{t}' in place, which is not a state of the graph")
+        elif users and len(readers[t]) > 1:
+            others = [n for n in readers[t] if n is not users[0]]
+            rep.error(f"{_who(users[0])} writes state '{t}' in place while {_who(others[0])} uses the value before: "
+                      f"let it use '{users[0].output}'")
+
     cyc = _cycle(graph, writers)
     if cyc:
         rep.error("dependence cycle through nodes " + " -> ".join(str(i) for i in cyc + cyc[:1]))
 
     returned = set(graph.outputs)
     for node in graph.nodes.values():
-        if not readers.get(node.output) and node.output not in returned:
+        if not readers.get(node.output) and node.output not in returned and node.op not in STATE_WRITERS:
             rep.warning(f"{_who(node)} is dead: nothing reads its output '{node.output}' and the graph does "
                         f"not return it")
     return rep.results
@@ -222,7 +236,7 @@ def _abi_fit(graph: Graph, node: Node, rep: _Report) -> None:
 @register_validator("execution_readiness", Phase.POST_RESOLVE_OPTIMIZE)
 def validate_execution_readiness(graph: Graph) -> list[ValidationResult]:
     rep = _Report("execution_readiness")
-    external = set(graph.inputs) | set(graph.constants)
+    external = graph.external
     for node in graph.nodes.values():
         if node.op.value >= FOLD_ONLY_BASE:
             rep.error(f"{_who(node)} is a fold-only op left in the graph; constant folding must remove it "

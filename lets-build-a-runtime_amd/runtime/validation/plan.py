@@ -68,7 +68,7 @@ def validate_memory_plan(plan: MemoryPlan) -> list[ValidationResult]:
         results.append(ValidationResult(who, sev, msg))
 
     graph = plan.graph
-    external = set(graph.inputs) | set(graph.constants)
+    external = graph.external
     read_back = len(plan.order)   # the host copies outputs back after the last step
     step_of_node = {node.id: s for s, node in enumerate(plan.order)}
 
