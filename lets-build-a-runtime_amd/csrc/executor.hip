@@ -748,6 +748,7 @@ int lbr_init(int device) {
         return LBR_ERR_NO_DEVICE;
     }
     HIP_TRY(mlp_prepare_device());
+    HIP_TRY(paged_prepare_device());
     // this device's copy of the no-allocation scratch array (see lbr_execute_noalloc)
     if (device < LBR_MAX_DEVICES && !g_scratch_dev[device]) {
         void* ptr = nullptr;

@@ -432,6 +432,8 @@ int decode_cache_write(const OpNode* n, Step* s);
 int decode_cache_read(const OpNode* n, Step* s);
 int decode_paged_attention(const OpNode* n, Step* s);
 int decode_verify_draft(const OpNode* n, Step* s);
+// Raises the paged attention kernels' dynamic LDS limit on the current device (lbr_init).
+hipError_t paged_prepare_device();
 // Bytes input k of a paged-cache or VERIFY_DRAFT node reads, -1 where its fields fix none.
 long long lbr_paged_input_bytes(const OpNode* n, int k);
 // Whether a decoded attention step can defer its store (its rows staged, then

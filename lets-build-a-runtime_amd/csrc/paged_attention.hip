@@ -1,123 +1,7 @@
-// paged_attention.hip — attention of a chunk of new tokens over the paged cache.
-//
-// Row i of sequence b attends to positions 0 .. start[b] + i; the rows of the query heads that share a K/V
-// head go together, row r of a K/V head being token r / G of its query head r % G.
-//
-// Products run on the fp16 matrix cores with 32-bit accumulators.  A stored K or V value is an fp16 number
-// exactly (int8, e4m3, float16) or the sum of two to 22 bits (float32, scaled into range by its row's power
-// of two); q and the weights are split into two fp16 numbers each, h = fp16(x), l = fp16(x − h), so that a
-// product of an exact value takes two MFMAs and one of two split ones three (the product of the low halves, below
-// 2^-22 of the whole, is left out).  Rows of q are brought to [2^14, 2^15) by a power of two first, and weights are
-// taken times the V row's scale over a running power of two, so that nothing overflows and the low halves
-// keep their bits.  The error against 64 bits is that of a 32-bit product (2e-7 .. 5e-7 of the outputs' norm).
-#include "paged_common.h"
-
-#include <math.h>
+// paged_attention.hip — attention over the paged cache: few rows a K/V head, and the choice between the kernels.
+#include "paged_attention.h"
 
 namespace {
-
-constexpr float LOG2E = 1.44269504088896340736f;
-
-struct PagedAttn {
-    PagedCache c;
-    const float* q;           // [B][H][S][hd]
-    float* out;
-    float* parts;             // partial results of split segments
-    int B, H, G, S;           // G: query heads of a K/V head
-    int G_m, G_s;             // divisor by G (lbr_fdiv)
-    int rows;                 // G · S: rows of a K/V head
-    float scale;              // of the scores, times log2 e
-    bool vec;                 // rows of q and out on 16-byte boundaries
-};
-
-// A sequence's rows and keys: count of rows 0 .. S, keys 0 .. the table's end (0 where start is negative).
-struct Span {
-    int start, count, keys;
-};
-__device__ __forceinline__ Span span_of(const PagedAttn& a, int b) {
-    Span s;
-    s.start = a.c.start[b];
-    s.count = min(max(a.c.count[b], 0), a.S);
-    const long long all = (long long)s.start + s.count, cap = (long long)a.c.wide << a.c.shift;
-    s.keys = s.start < 0 || s.count == 0 ? 0 : (int)min(all, cap);
-    return s;
-}
-
-// A row's result from its sum: zeros behind the sequence's rows, NaN where the table does not reach.
-__device__ __forceinline__ float row_value(const PagedAttn& a, const Span& s, int token, float v) {
-    if (token >= s.count) return 0.f;
-    return s.start < 0 || s.start + token >= ((long long)a.c.wide << a.c.shift) ? __uint_as_float(0x7fc00000u) : v;
-}
-
-// ---------------------------------------------------------------- fp16 operands
-
-__device__ __forceinline__ halfx2 to_half2(float x, float y) {
-    return __builtin_convertvector((floatx2{x, y}), halfx2);
-}
-
-// h + l of eight floats.
-__device__ __forceinline__ void split8(const float (&x)[8], halfx8& h, halfx8& l) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const halfx2 hi = to_half2(x[2 * k], x[2 * k + 1]);
-        const halfx2 lo = to_half2(x[2 * k] - (float)hi[0], x[2 * k + 1] - (float)hi[1]);
-        h[2 * k] = hi[0];
-        h[2 * k + 1] = hi[1];
-        l[2 * k] = lo[0];
-        l[2 * k + 1] = lo[1];
-    }
-}
-
-// Eight stored one-byte values (two words) as fp16.
-template <int TYPE>
-__device__ __forceinline__ halfx8 widen8(unsigned w0, unsigned w1) {
-    union {
-        halfx2 h[4];
-        halfx8 v;
-    } r;
-    const unsigned w[2] = {w0, w1};
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        if constexpr (TYPE == LBR_CACHE_I8) {
-            // byte + 128 under the exponent of 1024: 1024 + 128 + x, exactly
-            const unsigned u = w[k] ^ 0x80808080u;
-            const halfx2 bias = {(_Float16)-1152.f, (_Float16)-1152.f};
-            r.h[2 * k] = __builtin_bit_cast(halfx2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + bias;
-            r.h[2 * k + 1] = __builtin_bit_cast(halfx2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + bias;
-        } else {
-            r.h[2 * k] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[k], 1.0f, false);
-            r.h[2 * k + 1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[k], 1.0f, true);
-        }
-    }
-    return r.v;
-}
-
-// max / sum over the four lanes that hold the same row (lane ^ 16, lane ^ 32).
-__device__ __forceinline__ float quad_max(float v) {
-    const unsigned u = __float_as_uint(v);
-    auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const unsigned w = __float_as_uint(v);
-    auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float quad_sum(float v) {
-    const unsigned u = __float_as_uint(v);
-    auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    const unsigned w = __float_as_uint(v);
-    auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-__device__ __forceinline__ unsigned quad_max_bits(unsigned v) {
-    auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    v = max((unsigned)a[0], (unsigned)a[1]);
-    auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return max((unsigned)b[0], (unsigned)b[1]);
-}
-
-// Biased exponent of the power of two that brings a magnitude's bits into [2^14, 2^15), at most 2^127.
-__device__ __forceinline__ int up_exponent(unsigned bits) { return min(268 - max((int)(bits >> 23), 1), 254); }
 
 // ---------------------------------------------------------------- few rows: split over the keys
 //
@@ -609,23 +493,6 @@ long long split_ranges(const Step& s) {
 // Whether a segment can be longer than a step, and so cut.
 bool split_cuts(const Step& s) { return (s.i[6] << s.i[4]) > STEP_WG; }
 
-PagedAttn attn_args(const Step& s) {
-    PagedAttn a;
-    a.c = paged_cache(s);
-    a.q = (const float*)s.in[4];
-    a.out = (float*)s.out;
-    a.parts = (float*)s.ws;
-    a.B = (int)s.i[1];
-    a.H = (int)s.i[8];
-    a.S = (int)s.i[7];
-    a.G = a.H / a.c.heads;
-    lbr_fast_divisor((unsigned)a.G, &a.G_m, &a.G_s);
-    a.rows = a.G * a.S;
-    a.scale = s.f[0] * LOG2E;
-    a.vec = s.i[9] != 0;
-    return a;
-}
-
 template <int TYPE, int HD, int NR>
 void launch_split(const Step& s, hipStream_t st) {
     const PagedAttn a = attn_args(s);
@@ -644,83 +511,6 @@ step_fn split_rows(int nr) {
 template <int TYPE>
 step_fn split_for(int hd, int nr) {
     return hd <= 64 ? split_rows<TYPE, 64>(nr) : hd <= 128 ? split_rows<TYPE, 128>(nr) : split_rows<TYPE, 256>(nr);
-}
-
-constexpr int MAX_HD = 256;
-
-// One workgroup a row of Q: scores of 256 keys at a time, the running maximum and sum of the softmax
-// over them, and the weighted sum of the V rows, thread d holding column d.
-template <int TYPE>
-__global__ __launch_bounds__(256) void paged_rows(PagedCache c, const float* __restrict__ q, float* __restrict__ out,
-                                                  int H, int S, float scale) {
-    __shared__ float qs[MAX_HD], ps[256], red[4];
-    const int row = blockIdx.x % S, bh = blockIdx.x / S;
-    const int h = bh % H, b = bh / H, kvh = h / (H / c.heads);
-    const int tid = threadIdx.x;
-    const long long at = (long long)blockIdx.x * c.hd;
-    const int start = c.start[b], count = min(max(c.count[b], 0), S);
-    if (row >= count) {
-        if (tid < c.hd) out[at + tid] = 0.f;
-        return;
-    }
-    const long long keys = (long long)start + row + 1;
-    if (start < 0 || keys > ((long long)c.wide << c.shift)) {
-        if (tid < c.hd) out[at + tid] = __uint_as_float(0x7fc00000u);
-        return;
-    }
-    if (tid < c.hd) qs[tid] = q[at + tid] * scale;
-    constexpr int ES = cache_elem(TYPE);
-    const int page = 1 << c.shift;
-    auto value = [&](const char* p) {
-        if constexpr (TYPE == LBR_CACHE_F32) return *(const float*)p;
-        if constexpr (TYPE == LBR_CACHE_F16) return (float)*(const _Float16*)p;
-        if constexpr (TYPE == LBR_CACHE_I8) return (float)*(const signed char*)p;
-        if constexpr (TYPE == LBR_CACHE_E4M3)
-            return __builtin_amdgcn_cvt_f32_fp8((int)*(const unsigned char*)p, 0);
-    };
-    float m = -INFINITY, l = 0.f, o = 0.f;
-    for (long long k0 = 0; k0 < keys; k0 += 256) {
-        const long long key = k0 + tid;
-        __syncthreads();
-        float sc = -INFINITY;
-        if (key < keys) {
-            const char* head = cache_head(c, b, kvh, key);
-            const int slot = (int)key & (page - 1);
-            if (head) {
-                float dot = 0.f;
-                for (int d = 0; d < c.hd; ++d) dot += qs[d] * value(head + ((long long)slot * c.hdp + d) * ES);
-                sc = dot * ((const float*)(head + 2 * c.part))[slot];
-            } else {
-                sc = __uint_as_float(0x7fc00000u);
-            }
-        }
-        const bool nan = __syncthreads_or(sc != sc);
-        const float mx = fmaxf(m, block_max(sc, red));
-        const float p = nan ? __uint_as_float(0x7fc00000u) : expf(sc - mx);
-        ps[tid] = p;
-        const float sum = block_sum(p, red);
-        const float alpha = expf(m - mx);
-        l = l * alpha + sum;
-        o *= alpha;
-        m = mx;
-        if (tid < c.hd)
-            for (int j = 0; j < 256 && k0 + j < keys; ++j) {
-                const char* head = cache_head(c, b, kvh, k0 + j);
-                const int slot = (int)(k0 + j) & (page - 1);
-                if (!head) continue;
-                const float v = value(head + c.part + ((long long)(slot >> 3) * c.hdp + tid) * 8 * ES + (slot & 7) * ES);
-                o += ps[j] * (v * ((const float*)(head + 2 * c.part))[page + slot]);
-            }
-    }
-    if (tid < c.hd) out[at + tid] = o / l;
-}
-
-template <int TYPE>
-void launch_rows(const Step& s, hipStream_t st) {
-    const long long rows = s.i[1] * s.i[8] * s.i[7];
-    if (rows <= 0) return;
-    hipLaunchKernelGGL((paged_rows<TYPE>), dim3((unsigned)rows), dim3(256), 0, st, paged_cache(s),
-                       (const float*)s.in[4], (float*)s.out, (int)s.i[8], (int)s.i[7], s.f[0]);
 }
 
 }  // namespace
@@ -766,10 +556,14 @@ int decode_paged_attention(const OpNode* n, Step* s) {
         s->name = "paged_split";
         return LBR_OK;
     }
-    s->run = s->i[0] == LBR_CACHE_F32   ? launch_rows<LBR_CACHE_F32>
-             : s->i[0] == LBR_CACHE_F16 ? launch_rows<LBR_CACHE_F16>
-             : s->i[0] == LBR_CACHE_I8  ? launch_rows<LBR_CACHE_I8>
-                                        : launch_rows<LBR_CACHE_E4M3>;
-    s->name = "paged_attention_rows";
+    // grid: row tiles of all K/V heads
+    if (paged_row_tiles(*s) > ((1LL << 31) - 1) / (s->i[2] * (s->i[1] > 0 ? s->i[1] : 1))) {
+        lbr_set_error("paged_attention: %lld rows are more than one launch takes", node_total(n) / d[3]);
+        return LBR_ERR_INVALID;
+    }
+    s->i[10] = paged_tiles_splits(*s);
+    s->ws_bytes = paged_tiles_workspace(*s);
+    s->run = paged_tiles_launcher((int)s->i[0], hd);
+    s->name = "paged_tiles";
     return LBR_OK;
 }
