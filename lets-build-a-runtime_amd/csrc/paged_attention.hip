@@ -303,6 +303,7 @@ __global__ __launch_bounds__(256, 2) void paged_split(PagedAttn a) {
                 split8(p, ph[r], pl[r]);
                 const float f = __builtin_amdgcn_ldexpf(alpha, vnew - vup);
                 if (__any(f != 1.f)) {
+                    asm volatile("");   // a branch: done ahead of it, the products would need registers of their own
 #pragma unroll
                     for (int j = 0; j < ND; ++j) o[r][j] *= f;
                 }

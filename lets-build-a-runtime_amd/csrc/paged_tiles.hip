@@ -1,15 +1,16 @@
 // paged_tiles.hip — attention over the paged cache: chunks of more than 64 rows a K/V head.
 #include "paged_attention.h"
 
+#include <type_traits>
+
 namespace {
 
 // ---------------------------------------------------------------- many rows: tiles of rows and keys
 //
 // A workgroup takes 128 rows of a K/V head, 32 a wavefront, and goes over the keys in tiles of KT, double
-// buffered in LDS; S^T = K·Q^T and O^T = V^T·P^T as above, on 32×32×16 MFMAs.  K lies in LDS by chunks of eight columns,
-// [chunk][key], keys swizzled by the chunk, so that the reads (32 keys of a chunk) and the writes (16 chunks of a
-// key) both touch every bank once; V lies as in the cache, [group of 8 keys][column].  One-byte values are widened once on
-// their way into LDS, for all four wavefronts.  While a tile is computed the next one's loads are in
+// buffered in LDS; S^T = K·Q^T and O^T = V^T·P^T as for few rows, on 32×32×16 MFMAs.  V lies in LDS as in the cache,
+// [group of 8 keys][column].  float16 goes straight into LDS; one-byte values are widened, and floats split, once on
+// their way there for all four wavefronts.  While a tile is computed the next one's loads are in
 // flight.  A wavefront's 64 MFMAs a tile (head_dim 128, exact types) take 2048 cycles and the softmax of its 32 values
 // a lane about 1400 of the other unit's: two wavefronts a SIMD overlap the two.
 //
@@ -30,29 +31,36 @@ __device__ __forceinline__ int tile_keys(const PagedAttn& a, const Span& sp, int
     return sp.keys == 0 || first >= sp.count ? 0 : min(sp.start + min(last, sp.count - 1) + 1, sp.keys);
 }
 
-// (K/V head of a sequence, row tile) of a workgroup: the tiles with the most keys first, and with eight or a
-// multiple of eight heads all tiles of a head on one XCD, whose L2 then holds its keys for them.
-__device__ __forceinline__ void tile_of(int id, int tiles, int heads, int& bh, int& tile) {
-    if (heads % 8 == 0) {
-        const int at = id >> 3;
-        bh = at / tiles * 8 + (id & 7);
-        tile = tiles - 1 - at % tiles;
-    } else {
-        bh = id / tiles;
-        tile = tiles - 1 - id % tiles;
-    }
+// (K/V head of a sequence, row tile) of a workgroup: the tiles with the most keys first; with a multiple of
+// eight heads all tiles of a head on one XCD, whose L2 then holds its keys for them.  `fold`: all workgroups are
+// there at once, two a CU; the second half then goes from the fewest keys up, beside the first's most.
+__device__ __forceinline__ void tile_of(int id, int tiles, int heads, bool fold, int& bh, int& tile) {
+    const int lanes = heads % 8 == 0 ? 8 : 1, own = heads / lanes, all = own * tiles;
+    int at = id / lanes;
+    if (fold && at >= (all + 1) / 2) at = all - 1 - (at - (all + 1) / 2);
+    bh = at % own * lanes + id % lanes;
+    tile = tiles - 1 - at / own;
 }
 
+// K rows lie in LDS as chunks of eight columns, chunk ch of key k at place ch ^ swizzle(k): 16 keys' reads of a
+// chunk then lie in 16 different places of the 256 bytes that all banks make.
+template <int CH>
+__device__ __forceinline__ int swizzle(int key) { return CH == 8 ? key >> 1 & 7 : key & 15; }
+
 template <int TYPE, int HD>
-__global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void paged_tiles(PagedAttn a, int tiles) {
+__global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void paged_tiles(PagedAttn a, int tiles, bool fold) {
     constexpr int ES = cache_elem(TYPE);
     constexpr int PL = TYPE == LBR_CACHE_F32 ? 2 : 1;
     constexpr int KT = PL == 2 ? 32 : 64;       // keys a tile
+    constexpr int BK = KT / 4;                  // of a wavefront's loads
     constexpr int NB = KT / 32;                 // blocks of 32 keys
     constexpr int NK = HD / 16, ND = HD / 32;
+    constexpr int CH = HD / 8;                  // chunks of eight columns
     constexpr int PLANE = KT * HD;              // halves of a plane of K or V
-    constexpr int NL = KT * HD * ES / 16 / 256; // 16-byte loads a thread, of K and of V
-    static_assert(NL >= 1 && NL * 256 * 16 == KT * HD * ES, "a tile splits evenly over the threads");
+    constexpr bool DMA = TYPE == LBR_CACHE_F16; // straight into LDS
+    constexpr int KU = HD * ES / 16, VU = HD * ES / 2;   // 16-byte units of a K row, of a V group
+    constexpr int NL = BK * KU / 64;            // 16-byte loads a thread, of K and of V
+    static_assert(NL >= 1 && NL * 64 == BK * KU && BK * KU == BK / 8 * VU, "a wavefront's keys split evenly over its lanes");
     extern __shared__ __attribute__((aligned(16))) char lds[];
     // [2 buffers][K planes, V planes, ks, vs], then the tiles' largest V scales
     constexpr int BUF = 2 * PL * PLANE * 2 + 2 * KT * 4;
@@ -62,7 +70,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void paged_tiles(PagedAttn a
     const PagedCache& c = a.c;
     const int mask = (1 << c.shift) - 1;
     int bh, tile;
-    tile_of(blockIdx.x, tiles, a.B * c.heads, bh, tile);
+    tile_of(blockIdx.x, tiles, a.B * c.heads, fold, bh, tile);
     const int b = bh / c.heads, h = bh % c.heads;
     const Span sp = span_of(a, b);
     const int keys = tile_keys(a, sp, tile);
@@ -122,118 +130,125 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void paged_tiles(PagedAttn a
         }
     }
 
-    // a thread's 16-byte loads of a tile: K row and columns, V group and columns; each lies in one block of 16
-    // positions, the same for the whole wavefront, and so in one page
-    uint4 kr[NL], vr[NL];
-    float ksr = 0.f, vsr = 0.f;
-    constexpr int KU = HD * ES / 16, VU = HD * ES / 2;   // 16-byte units of a K row, of a V group
-    int base_key = 0;
-    auto head_of = [&](int key, bool& bad) {   // key wave-uniform, below the end
-        const int page = c.table[(long long)b * c.wide + (key >> c.shift)];
-        bad = page < 0 || page >= c.pages;
-        return c.base + (bad ? 0 : page) * c.page_bytes + (long long)h * c.head_bytes;
-    };
-    auto load = [&](int t) {
-        base_key = t * KT;
+    // Loads of a tile.  A wavefront takes BK keys, which share a block of 16 positions and so a page: K rows and V
+    // groups in 16-byte units, past the page's range (which reads as zero) for columns that the rows do not have,
+    // groups behind the end and pages that are none.
+    typedef const __attribute__((address_space(4))) int* Table;
+    const Table table = (Table)(c.table + (long long)b * c.wide);
+    const int own = wave * BK;                            // the wavefront's first key in a tile
+    auto page_of = [&](int t) { return table[min(t * KT + own, keys - 1) >> c.shift]; };
+    constexpr unsigned NONE = 0x7ffffff0u;
+    unsigned koff[NL], voff[NL];
+    int kdst[NL];                                         // halves, in the K plane
 #pragma unroll
-        for (int u = 0; u < NL; ++u) {
-            const int unit = u * 256 + tid;
-            {
-                const int r = unit / KU, col = unit % KU * (16 / ES);
-                const int blk = __builtin_amdgcn_readfirstlane(r >> 4);
-                const int key0 = min(base_key + blk * 16, (keys - 1) & ~15);
-                bool bad;
-                const char* const hd = head_of(key0, bad);
-                kr[u] = *(const uint4*)(hd + ((long long)(key0 & mask) + (r & 15)) * c.hdp * ES + (col < c.hdp ? col : 0) * ES);
+    for (int u = 0; u < NL; ++u) {
+        const int unit = u * 64 + lane;
+        if constexpr (DMA) {   // LDS is filled in order: lane l's unit is the one that belongs there
+            const int r = unit / CH, ch = unit % CH ^ swizzle<CH>(own + r);
+            koff[u] = ch * 8 < c.hdp ? (unsigned)(r * c.hdp + ch * 8) * ES : NONE;
+        } else {
+            const int r = unit / KU, col = unit % KU * (16 / ES);
+            koff[u] = col < c.hdp ? (unsigned)(r * c.hdp + col) * ES : NONE;
+            kdst[u] = (own + r) * HD + ((col / 8) ^ swizzle<CH>(own + r)) * 8 + col % 8;
+        }
+        const int gr = unit / VU, at = unit % VU * 16;
+        voff[u] = at < c.hdp * 8 * ES ? (unsigned)(c.part + gr * 8 * c.hdp * ES + at) : NONE;
+    }
+    uint4 kr[NL], vr[NL];
+    float scale_r = 0.f;
+    float* const tops = (float*)(lds + 2 * BUF);          // [2][4]: the largest V scale of each wavefront's keys
+    auto load = [&](int t, int page, int buf) {
+        const int key0 = t * KT + own;
+        const bool bad = page < 0 || page >= c.pages;
+        const char* const hd = c.base + (bad ? 0 : page) * c.page_bytes + (long long)h * c.head_bytes;
+        const int slot = min(key0, keys - 1) & mask & ~(BK - 1);
+        const bool none = bad || key0 >= keys;
+        const __amdgpu_buffer_rsrc_t rs =
+            __builtin_amdgcn_make_buffer_rsrc((void*)hd, (short)0, none ? 0 : c.head_bytes, 0x00020000);
+        const unsigned soff = (unsigned)(slot * c.hdp * ES);
+        if constexpr (DMA) {
+            _Float16* const kp = (_Float16*)(lds + buf * BUF) + own * HD;
+            _Float16* const vp = (_Float16*)(lds + buf * BUF) + PLANE + own * HD;
+#pragma unroll
+            for (int u = 0; u < NL; ++u) {
+                lbr_dma16(rs, (float*)(kp + u * 512), koff[u], soff);
+                const bool there = key0 + (u * 64 + lane) / VU * 8 < keys;
+                lbr_dma16(rs, (float*)(vp + u * 512), there ? voff[u] : NONE, soff);
             }
-            {
-                const int gr = unit / VU, at = unit % VU * 16;   // byte of the group's [column][8]
-                const int blk = __builtin_amdgcn_readfirstlane(gr >> 1);
-                const int key0 = min(base_key + blk * 16, (keys - 1) & ~15);
-                bool bad;
-                const char* const hd = head_of(key0, bad);
-                const char* const p = hd + c.part + ((long long)(key0 & mask) + (gr & 1) * 8) * c.hdp * ES;
-                uint4 v = *(const uint4*)(p + (at < c.hdp * 8 * ES ? at : 0));
-                // positions behind the end, and pages that are none, hold anything
-                const int keep = bad ? 0 : keys - (base_key + gr * 8);
-                if (bad || base_key + KT > keys) {
+        } else {
+#pragma unroll
+            for (int u = 0; u < NL; ++u) {
+                kr[u] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, koff[u], soff, 0));
+                const bool there = key0 + (u * 64 + lane) / VU * 8 < keys;
+                vr[u] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, there ? voff[u] : NONE, soff, 0));
+            }
+        }
+        // scales: lanes 0 .. BK−1 of K rows, BK .. 2·BK−1 of V rows
+        const int k = key0 + (lane & (BK - 1));
+        const float* const sc = (const float*)(hd + 2 * c.part) + (lane & BK ? mask + 1 : 0);
+        scale_r = sc[min(k, keys - 1) & mask];
+        if (bad) scale_r = __uint_as_float(0x7fc00000u);
+        if (lane & BK && k >= keys) scale_r = 0.f;
+    };
+    auto store = [&](int t, int buf) {
+        _Float16* const kp = (_Float16*)(lds + buf * BUF);
+        _Float16* const vp = kp + PL * PLANE;
+        const int key0 = t * KT + own;
+        if constexpr (!DMA) {
+            // the end lies inside a group: what is behind it may be anything
+            if (key0 < keys && key0 + BK > keys && (keys & 7)) {
+#pragma unroll
+                for (int u = 0; u < NL; ++u) {
+                    const int keep = keys - (key0 + (u * 64 + lane) / VU * 8);
                     if (ES == 4) {
-                        const int k0 = at / 4 % 8;
-                        if (k0 >= keep) v.x = 0;
-                        if (k0 + 1 >= keep) v.y = 0;
-                        if (k0 + 2 >= keep) v.z = 0;
-                        if (k0 + 3 >= keep) v.w = 0;
-                    } else if (ES == 2) {
-                        if (keep < 1) v.x = 0; else if (keep < 2) v.x &= 0xffffu;
-                        if (keep < 3) v.y = 0; else if (keep < 4) v.y &= 0xffffu;
-                        if (keep < 5) v.z = 0; else if (keep < 6) v.z &= 0xffffu;
-                        if (keep < 7) v.w = 0; else if (keep < 8) v.w &= 0xffffu;
+                        const int k0 = lane % 2 * 4;   // four of a column's eight keys
+                        if (k0 >= keep) vr[u].x = 0;
+                        if (k0 + 1 >= keep) vr[u].y = 0;
+                        if (k0 + 2 >= keep) vr[u].z = 0;
+                        if (k0 + 3 >= keep) vr[u].w = 0;
                     } else {
                         const unsigned lo = keep >= 4 ? ~0u : keep <= 0 ? 0u : (1u << (8 * keep)) - 1u;
                         const unsigned hi = keep >= 8 ? ~0u : keep <= 4 ? 0u : (1u << (8 * (keep - 4))) - 1u;
-                        v.x &= lo;
-                        v.y &= hi;
-                        v.z &= lo;
-                        v.w &= hi;
+                        vr[u].x &= lo;
+                        vr[u].y &= hi;
+                        vr[u].z &= lo;
+                        vr[u].w &= hi;
                     }
                 }
-                vr[u] = v;
             }
-        }
-        if (tid < KT) {   // the scales
-            const int key = base_key + tid, k1 = min(key, keys - 1);
-            const int page = c.table[(long long)b * c.wide + (k1 >> c.shift)];
-            const bool bad = page < 0 || page >= c.pages;
-            const float* const sc = (const float*)(c.base + (bad ? 0 : page) * c.page_bytes + (long long)h * c.head_bytes + 2 * c.part);
-            ksr = bad ? __uint_as_float(0x7fc00000u) : sc[k1 & mask];
-            vsr = key >= keys ? 0.f : bad ? __uint_as_float(0x7fc00000u) : sc[mask + 1 + (k1 & mask)];
-        }
-    };
-    float* const tops = (float*)(lds + 2 * BUF);
-    auto store = [&](int buf) {
-        _Float16* const kp = (_Float16*)(lds + buf * BUF);
-        _Float16* const vp = kp + PL * PLANE;
-        float* const ks = (float*)(lds + buf * BUF + 2 * PL * PLANE * 2);
 #pragma unroll
-        for (int u = 0; u < NL; ++u) {
-            const int unit = u * 256 + tid;
-            const int r = unit / KU;
-            auto slot = [&](int ch) { return (ch * KT + (r ^ (ch & 15))) * 8; };
-            if constexpr (TYPE == LBR_CACHE_F32) {
-                const int ch = unit % KU / 2, part = unit % 2 * 4;   // four of the eight columns
-                const int vat = unit * 4;                            // [group][column][8], four of the eight keys
-                const float fk[4] = {__uint_as_float(kr[u].x), __uint_as_float(kr[u].y), __uint_as_float(kr[u].z), __uint_as_float(kr[u].w)};
-                const float fv[4] = {__uint_as_float(vr[u].x), __uint_as_float(vr[u].y), __uint_as_float(vr[u].z), __uint_as_float(vr[u].w)};
-                halfx4 hk, lk, hv, lv;
+            for (int u = 0; u < NL; ++u) {
+                _Float16* const vd = vp + own * HD + (u * 64 + lane) * (16 / ES);
+                if constexpr (TYPE == LBR_CACHE_F32) {
+                    const float fk[4] = {__uint_as_float(kr[u].x), __uint_as_float(kr[u].y), __uint_as_float(kr[u].z), __uint_as_float(kr[u].w)};
+                    const float fv[4] = {__uint_as_float(vr[u].x), __uint_as_float(vr[u].y), __uint_as_float(vr[u].z), __uint_as_float(vr[u].w)};
+                    halfx4 hk, lk, hv, lv;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    hk[e] = (_Float16)fk[e];
-                    lk[e] = (_Float16)(fk[e] - (float)hk[e]);
-                    hv[e] = (_Float16)fv[e];
-                    lv[e] = (_Float16)(fv[e] - (float)hv[e]);
+                    for (int e = 0; e < 4; ++e) {
+                        hk[e] = (_Float16)fk[e];
+                        lk[e] = (_Float16)(fk[e] - (float)hk[e]);
+                        hv[e] = (_Float16)fv[e];
+                        lv[e] = (_Float16)(fv[e] - (float)hv[e]);
+                    }
+                    *(halfx4*)(kp + kdst[u]) = hk;
+                    *(halfx4*)(kp + PLANE + kdst[u]) = lk;
+                    *(halfx4*)vd = hv;
+                    *(halfx4*)(vd + PLANE) = lv;
+                } else if constexpr (ES == 1) {
+                    *(halfx8*)(kp + kdst[u]) = widen8<TYPE>(kr[u].x, kr[u].y);
+                    *(halfx8*)(kp + (kdst[u] ^ 8)) = widen8<TYPE>(kr[u].z, kr[u].w);   // the next chunk
+                    *(halfx8*)vd = widen8<TYPE>(vr[u].x, vr[u].y);
+                    *(halfx8*)(vd + 8) = widen8<TYPE>(vr[u].z, vr[u].w);
                 }
-                *(halfx4*)(kp + slot(ch) + part) = hk;
-                *(halfx4*)(kp + PLANE + slot(ch) + part) = lk;
-                *(halfx4*)(vp + vat) = hv;
-                *(halfx4*)(vp + PLANE + vat) = lv;
-            } else if constexpr (TYPE == LBR_CACHE_F16) {
-                *(halfx8*)(kp + slot(unit % KU)) = __builtin_bit_cast(halfx8, kr[u]);
-                *(halfx8*)(vp + unit * 8) = __builtin_bit_cast(halfx8, vr[u]);
-            } else {
-                const int ch = unit % KU * 2;
-                *(halfx8*)(kp + slot(ch)) = widen8<TYPE>(kr[u].x, kr[u].y);
-                *(halfx8*)(kp + slot(ch + 1)) = widen8<TYPE>(kr[u].z, kr[u].w);
-                *(halfx8*)(vp + unit * 16) = widen8<TYPE>(vr[u].x, vr[u].y);
-                *(halfx8*)(vp + unit * 16 + 8) = widen8<TYPE>(vr[u].z, vr[u].w);
             }
         }
-        if (tid < KT) {
-            ks[tid] = __builtin_amdgcn_ldexpf(ksr, -KS_UP);
-            ks[KT + tid] = vsr;
-            float top = fmaxf(vsr, 0.f);
-            for (int o = KT / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, KT));
-            if (tid == 0) tops[buf] = top;
-        }
+        float* const sc = (float*)(lds + buf * BUF + 2 * PL * PLANE * 2);
+        if (lane < BK) sc[own + lane] = __builtin_amdgcn_ldexpf(scale_r, -KS_UP);
+        else if (lane < 2 * BK) sc[KT + own + lane - BK] = scale_r;
+        float top = lane & BK ? fmaxf(scale_r, 0.f) : 0.f;
+#pragma unroll
+        for (int o = 1; o <= BK; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+        if (lane == 0) tops[buf * 4 + wave] = top;
     };
 
     floatx16 o[ND];
@@ -244,114 +259,138 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void paged_tiles(PagedAttn a
     float m = -INFINITY, l = 0.f;
     int vup = VUP_MOST;   // biased exponent of the power of two that weights are taken by (see the sums below)
 
-    if (t0 < t1) {
-        load(t0);
-        store(0);
-    }
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-        const int buf = (t - t0) & 1;
-        if (t + 1 < t1) load(t + 1);
+    // block row m of the MFMA is key (m / 16)·16 + (m / 4 % 2)·8 + (m / 8 % 2)·4 + m % 4 of its 32
+    const int kk = (n >> 4) * 16 + (n >> 2 & 1) * 8 + (n >> 3 & 1) * 4 + (n & 3);
+    // EDGE: some row of the workgroup ends in the tile
+    auto compute = [&](int t, int buf, auto edge) {
+        constexpr bool EDGE = decltype(edge)::value;
         const int k0 = t * KT;
-        if (k0 <= wave_last) {
-            const _Float16* const kp = (const _Float16*)(lds + buf * BUF);
-            const _Float16* const vp = kp + PL * PLANE;
-            const float* const ks = (const float*)(lds + buf * BUF + 2 * PL * PLANE * 2);
-            const float* const vs = ks + KT;
-            floatx16 s[NB];
-            // block row m of the MFMA is key (m / 16)·16 + (m / 4 % 2)·8 + (m / 8 % 2)·4 + m % 4
-            const int kk = (n >> 4) * 16 + (n >> 2 & 1) * 8 + (n >> 3 & 1) * 4 + (n & 3);
+        const _Float16* const kp = (const _Float16*)(lds + buf * BUF);
+        const _Float16* const vp = kp + PL * PLANE;
+        const float* const ks = (const float*)(lds + buf * BUF + 2 * PL * PLANE * 2);
+        const float* const vs = ks + KT;
+        floatx16 s[NB];
 #pragma unroll
-            for (int q = 0; q < NB; ++q) {
+        for (int q = 0; q < NB; ++q) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[q][i] = 0.f;
+            for (int i = 0; i < 16; ++i) s[q][i] = 0.f;
 #pragma unroll
-                for (int j = 0; j < NK; ++j) {
-                    const int ch = 2 * j + hf;
-                    const int at = (ch * KT + ((q * 32 + kk) ^ (ch & 15))) * 8;
-                    const halfx8 kh = *(const halfx8*)(kp + at);
-                    s[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[j], s[q], 0, 0, 0);
-                    if constexpr (PL == 2) {
-                        const halfx8 kl = *(const halfx8*)(kp + PLANE + at);
-                        s[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[j], s[q], 0, 0, 0);
-                    }
-                    s[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[j], s[q], 0, 0, 0);
+            for (int j = 0; j < NK; ++j) {
+                const int at = (q * 32 + kk) * HD + ((2 * j + hf) ^ swizzle<CH>(kk)) * 8;   // the swizzle has period 16
+                const halfx8 kh = *(const halfx8*)(kp + at);
+                s[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[j], s[q], 0, 0, 0);
+                if constexpr (PL == 2) {
+                    const halfx8 kl = *(const halfx8*)(kp + PLANE + at);
+                    s[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[j], s[q], 0, 0, 0);
+                }
+                s[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[j], s[q], 0, 0, 0);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);   // or reads hoisted over the phases spill
+        // scores (over qs), the row's maximum; accumulator i of block q is key 32·q + (i / 8)·16 + 8·hf + i % 8
+        float top = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < NB; ++q)
+#pragma unroll
+            for (int i8 = 0; i8 < 16; i8 += 4) {
+                const int key = 32 * q + (i8 >> 3) * 16 + 8 * hf + (i8 & 7);
+                const floatx4 sc = *(const floatx4*)(ks + key);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float v = s[q][i8 + e] * sc[e];
+                    if (EDGE && k0 + key + e > last) v = -INFINITY;
+                    s[q][i8 + e] = v;
+                    top = fmaxf(top, v);
                 }
             }
-            // scores (over qs), the row's maximum; accumulator i of block q is key 32·q + (i / 8)·16 + 8·hf + i % 8
-            float top = -INFINITY;
-            const bool edge = k0 + KT - 1 > sp.start || k0 + KT > keys;   // some row ends in this tile
+        {
+            const unsigned u = __float_as_uint(top);
+            auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+            top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * qs;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // Weights are taken times 2^(vup − 127), which brings the largest V scale so far to [2^14, 2^15): their
+        // products with the scales then fit fp16, and the sums carry the same factor.
+        const floatx4 vt = *(const floatx4*)(tops + buf * 4);
+        const float vtop = fmaxf(fmaxf(vt[0], vt[1]), fmaxf(vt[2], vt[3]));
+        const int vnew = __builtin_amdgcn_readfirstlane(min(vup, min(up_exponent(__float_as_uint(vtop)), VUP_MOST)));
+        const float mx = fmaxf(m, top);
+        const float base = mx == -INFINITY ? 0.f : mx;
+        const float f = __builtin_amdgcn_exp2f(m - base + (float)(vnew - vup));
+        const float sub = base - (float)(vnew - 127);
+        m = mx;
+        vup = vnew;
+        float sum = 0.f;
+        halfx8 ph[2 * NB], pl[2 * NB];
 #pragma unroll
-            for (int q = 0; q < NB; ++q)
+        for (int q = 0; q < 2 * NB; ++q) {
+            float p[8];
 #pragma unroll
-                for (int i8 = 0; i8 < 16; i8 += 4) {
-                    const int key = 32 * q + (i8 >> 3) * 16 + 8 * hf + (i8 & 7);
-                    const floatx4 sc = *(const floatx4*)(ks + key);
+            for (int i4 = 0; i4 < 8; i4 += 4) {
+                const floatx4 sc = *(const floatx4*)(vs + 16 * q + 8 * hf + i4);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float v = s[q][i8 + e] * sc[e];
-                        if (edge && k0 + key + e > last) v = -INFINITY;
-                        s[q][i8 + e] = v;
-                        top = fmaxf(top, v);
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    const float v = s[q >> 1][(q & 1) * 8 + i4 + e];
+                    const float w = __builtin_amdgcn_exp2f(fmaf(v, qs, -sub));
+                    sum += w;
+                    p[i4 + e] = w * sc[e];
+                    if (EDGE && v == -INFINITY) p[i4 + e] = 0.f;   // no weight, whatever the V row holds
                 }
-            {
-                const unsigned u = __float_as_uint(top);
-                auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-                top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * qs;
             }
-            // Weights are taken times 2^(vup − 127), which brings the largest V scale so far to [2^14, 2^15): their
-            // products with the scales then fit fp16, and the sums carry the same factor.
-            const int vnew = __builtin_amdgcn_readfirstlane(min(vup, min(up_exponent(__float_as_uint(tops[buf])), VUP_MOST)));
-            const float mx = fmaxf(m, top);
-            const float base = mx == -INFINITY ? 0.f : mx;
-            const float f = __builtin_amdgcn_exp2f(m - base + (float)(vnew - vup));
-            const float sub = base - (float)(vnew - 127);
-            m = mx;
-            vup = vnew;
-            float sum = 0.f;
-            halfx8 ph[2 * NB], pl[2 * NB];
-#pragma unroll
-            for (int q = 0; q < 2 * NB; ++q) {
-                float p[8];
-#pragma unroll
-                for (int i4 = 0; i4 < 8; i4 += 4) {
-                    const floatx4 sc = *(const floatx4*)(vs + 16 * q + 8 * hf + i4);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float v = s[q >> 1][(q & 1) * 8 + i4 + e];
-                        const float w = __builtin_amdgcn_exp2f(fmaf(v, qs, -sub));
-                        sum += w;
-                        p[i4 + e] = w * sc[e];
-                        if (edge && v == -INFINITY) p[i4 + e] = 0.f;   // no weight, whatever the V row holds
-                    }
-                }
-                split8(p, ph[q], pl[q]);
-            }
-            l = l * f + sum;
-            if (__any(f != 1.f)) {
-#pragma unroll
-                for (int j = 0; j < ND; ++j)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[j][i] *= f;
-            }
+            split8(p, ph[q], pl[q]);
+        }
+        l = l * f + sum;
+        if (__any(f != 1.f)) {
+            asm volatile("");   // a branch: done ahead of it, the products would need registers of their own
 #pragma unroll
             for (int j = 0; j < ND; ++j)
 #pragma unroll
-                for (int q = 0; q < 2 * NB; ++q) {
-                    const int at = ((2 * q + hf) * HD + 32 * j + n) * 8;
-                    const halfx8 vh = *(const halfx8*)(vp + at);
-                    o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[q], o[j], 0, 0, 0);
-                    if constexpr (PL == 2) {
-                        const halfx8 vl = *(const halfx8*)(vp + PLANE + at);
-                        o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[q], o[j], 0, 0, 0);
-                    }
-                    o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[q], o[j], 0, 0, 0);
-                }
+                for (int i = 0; i < 16; ++i) o[j][i] *= f;
         }
-        if (t + 1 < t1) store(buf ^ 1);
-        __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < ND; ++j)
+#pragma unroll
+            for (int q = 0; q < 2 * NB; ++q) {
+                const int at = ((2 * q + hf) * HD + 32 * j + n) * 8;
+                const halfx8 vh = *(const halfx8*)(vp + at);
+                o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[q], o[j], 0, 0, 0);
+                if constexpr (PL == 2) {
+                    const halfx8 vl = *(const halfx8*)(vp + PLANE + at);
+                    o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[q], o[j], 0, 0, 0);
+                }
+                o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[q], o[j], 0, 0, 0);
+            }
+    };
+
+    int page = 0;
+    if (t0 < t1) {
+        load(t0, page_of(t0), 0);
+        if (t0 + 1 < t1) page = page_of(t0 + 1);
+        store(t0, 0);
     }
+    if (DMA) __builtin_amdgcn_s_waitcnt(lbr_waitcnt_vm(0));
+    __syncthreads();
+    auto step = [&](int t, auto edge) {
+        const int buf = (t - t0) & 1;
+        if (DMA && decltype(edge)::value && t * KT + KT > keys && (keys & 7)) {
+            // the end lies inside a group of V: what is behind it may be anything
+            _Float16* const vp = (_Float16*)(lds + buf * BUF) + PLANE + (keys - t * KT) / 8 * 8 * HD;
+            for (int at = tid; at < HD * 8; at += 256)
+                if (at % 8 >= (keys & 7)) vp[at] = (_Float16)0.f;
+            __syncthreads();
+        }
+        if (t + 1 < t1) load(t + 1, page, buf ^ 1);
+        if (t + 2 < t1) page = page_of(t + 2);
+        if (t * KT <= wave_last) compute(t, buf, edge);
+        if (t + 1 < t1) store(t + 1, buf ^ 1);
+        if (DMA) __builtin_amdgcn_s_waitcnt(lbr_waitcnt_vm(0));
+        __syncthreads();
+    };
+    // tiles that all rows of the workgroup reach to their end, then the others
+    const int te = min(t1, max(t0, (min(sp.start, keys - 1) + 1) / KT));
+    for (int t = t0; t < te; ++t) step(t, std::false_type());
+    for (int t = te; t < t1; ++t) step(t, std::true_type());
 
     {
         const unsigned u = __float_as_uint(l);
@@ -389,11 +428,11 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void paged_tiles(PagedAttn a
 
 // Joins the ranges of the keys: one workgroup eight rows of a workgroup of paged_tiles.
 template <int HD>
-__global__ __launch_bounds__(256) void paged_tiles_merge(PagedAttn a, int tiles, int splits) {
+__global__ __launch_bounds__(256) void paged_tiles_merge(PagedAttn a, int tiles, int splits, bool fold) {
     constexpr int LANES = HD / 4, EACH = 256 / LANES;
     const PagedCache& c = a.c;
     int bh, tile;
-    tile_of(blockIdx.x, tiles, a.B * c.heads, bh, tile);
+    tile_of(blockIdx.x, tiles, a.B * c.heads, fold, bh, tile);
     const int b = bh / c.heads, h = bh % c.heads;
     const int r = blockIdx.y * EACH + threadIdx.x / LANES, row = tile * ROWS_WG + r, col = threadIdx.x % LANES * 4;
     if (row >= a.rows) return;
@@ -421,7 +460,7 @@ __global__ __launch_bounds__(256) void paged_tiles_merge(PagedAttn a, int tiles,
 template <int TYPE, int HD>
 constexpr size_t tiles_lds() {
     constexpr int pl = TYPE == LBR_CACHE_F32 ? 2 : 1, kt = pl == 2 ? 32 : 64;
-    return 2 * (2 * pl * kt * HD * 2 + 2 * kt * 4) + 16;
+    return 2 * (2 * pl * kt * HD * 2 + 2 * kt * 4) + 32;
 }
 
 template <int TYPE, int HD>
@@ -431,9 +470,10 @@ void launch_tiles(const Step& s, hipStream_t st) {
     const unsigned wgs = (unsigned)(tiles * s.i[1] * s.i[2]);
     if (!wgs) return;
     const unsigned lds = (unsigned)tiles_lds<TYPE, HD>();
-    hipLaunchKernelGGL((paged_tiles<TYPE, HD>), dim3(wgs, (unsigned)splits), dim3(256), lds, st, a, tiles);
+    const bool fold = splits == 1 && wgs <= 2u * (unsigned)lbr_device_cus();
+    hipLaunchKernelGGL((paged_tiles<TYPE, HD>), dim3(wgs, (unsigned)splits), dim3(256), lds, st, a, tiles, fold);
     if (splits > 1)
-        hipLaunchKernelGGL((paged_tiles_merge<HD>), dim3(wgs, ROWS_WG * (HD / 4) / 256), dim3(256), 0, st, a, tiles, splits);
+        hipLaunchKernelGGL((paged_tiles_merge<HD>), dim3(wgs, ROWS_WG * (HD / 4) / 256), dim3(256), 0, st, a, tiles, splits, fold);
 }
 
 template <int TYPE>
