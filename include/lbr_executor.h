@@ -165,7 +165,9 @@ int lbr_execute_noalloc(const OpNode* nodes, int n_nodes);
 /* Plans: validate and decode the node array once; launches reuse the
  * decoded kernel arguments.  With use_graph != 0 the launch sequence is
  * captured into a hipGraph at creation and every lbr_plan_launch replays it
- * (the device pointers in the nodes must stay valid and unchanged). */
+ * (the device pointers in the nodes must stay valid and unchanged); plans of
+ * at most three kernel steps, which a replay would slow down, are launched
+ * kernel by kernel all the same. */
 typedef struct lbr_plan lbr_plan;
 int lbr_plan_create(const OpNode* nodes, int n_nodes, int use_graph,
                     lbr_plan** out_plan);

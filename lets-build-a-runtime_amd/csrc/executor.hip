@@ -686,6 +686,11 @@ static int check_kernels(const lbr_plan& p) {
     return LBR_OK;
 }
 
+// Plans of at most this many kernel steps are launched kernel by kernel: a hipGraph replay costs the host 12-18 µs
+// whatever it holds, a launch 3.7 (a step has one or two), and puts 4-5 µs between replays that follow each other on
+// the device.  One step: 16.7 µs a pass replayed, 7.7 launched; two, 17.3 and 9.9; one of 63 µs of device time, 67 and 63.
+constexpr size_t DIRECT_STEPS = 3;
+
 static int create_plan(const OpNode* nodes, int n_nodes, int use_graph, bool fuse, const void* const* live_ptr,
                        const size_t* live_bytes, int n_live, lbr_plan** out_plan) {
     lbr_plan* p = new lbr_plan();
@@ -707,7 +712,7 @@ static int create_plan(const OpNode* nodes, int n_nodes, int use_graph, bool fus
         free_plan(p);
         return rc;
     }
-    if (use_graph && !p->steps.empty()) {
+    if (use_graph && p->steps.size() > DIRECT_STEPS) {
         hipError_t e = hipStreamBeginCapture(g_stream, hipStreamCaptureModeThreadLocal);
         if (e == hipSuccess) {
             run_steps(p->steps, g_stream);
