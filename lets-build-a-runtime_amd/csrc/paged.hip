@@ -1,12 +1,12 @@
 // paged.hip — the paged key/value cache: writing a chunk's rows with their scales, and reading
 // positions back (layout and types: paged_common.h).
 //
-// Both move rows at memory speed.  A wavefront takes eight positions that share a V group of
-// one head: lane (r, c) = (lane / 8, lane % 8) holds 8-column chunks c, c + 8, ... of position r's K and V
-// rows, so that K rows are 16-byte accesses and a row's largest magnitude is a reduction over eight lanes.
-// V changes its order, [8][hdp] to [hdp][8], through 8·hdp elements of LDS that only its wavefront
-// touches; a group that the chunk covers only in part is written element by element, its other
-// positions left alone.
+// Both move rows at memory speed.  A wavefront takes eight positions that share a V group of one head, in
+// the fp32 tensors eight rows in a row: LPR lanes a row hold four columns each, so that an access of the
+// wavefront is 1 KiB in a row there (lanes of eight columns, two accesses of every other 16 bytes, took 36 µs for
+// 127 MB read back, against 26.6), and a row's largest magnitude is a reduction over LPR lanes.  V changes its order,
+// [8][hdp] to [hdp][8], through 8·hdp elements of LDS that only its wavefront touches; a group that the chunk covers
+// only in part is written element by element, its other positions left alone.
 #include "paged_common.h"
 
 #include <math.h>
@@ -48,56 +48,56 @@ __device__ __forceinline__ float row_scale(unsigned amax) {
 // A value's stored bytes as the cache and the LDS stage hold them; both are read back in other widths.
 typedef unsigned __attribute__((may_alias)) word;
 typedef unsigned short __attribute__((may_alias)) word2;
+typedef uint2 __attribute__((may_alias)) word8;
 typedef uint4 __attribute__((may_alias)) word16;
 
-// Eight stored values: two (one-byte types) to eight words.
+// Four neighbouring values of a row as stored: one word to four.
 template <int TYPE>
-struct alignas(cache_elem(TYPE) == 1 ? 8 : 16) Chunk {
+struct Quad {
     static constexpr int ES = cache_elem(TYPE);
-    unsigned w[2 * ES];
+    unsigned w[ES];
 
     __device__ __forceinline__ void load(const char* p) {
         if constexpr (ES == 1) {
-            w[0] = ((const word*)p)[0];
-            w[1] = ((const word*)p)[1];
+            w[0] = *(const word*)p;
+        } else if constexpr (ES == 2) {
+            const uint2 v = *(const word8*)p;
+            w[0] = v.x;
+            w[1] = v.y;
         } else {
-#pragma unroll
-            for (int k = 0; k < ES / 2; ++k) {
-                const uint4 v = ((const word16*)p)[k];
-                w[4 * k] = v.x; w[4 * k + 1] = v.y; w[4 * k + 2] = v.z; w[4 * k + 3] = v.w;
-            }
+            const uint4 v = *(const word16*)p;
+            w[0] = v.x;
+            w[1] = v.y;
+            w[2] = v.z;
+            w[3] = v.w;
         }
     }
     __device__ __forceinline__ void store(char* p) const {
-        if constexpr (ES == 1) {
-            *(uint2 __attribute__((may_alias))*)p = make_uint2(w[0], w[1]);
-        } else {
-#pragma unroll
-            for (int k = 0; k < ES / 2; ++k)
-                ((word16*)p)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-        }
+        if constexpr (ES == 1) *(word*)p = w[0];
+        else if constexpr (ES == 2) *(word8*)p = make_uint2(w[0], w[1]);
+        else *(word16*)p = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    // Element q alone, to or from its place.
+    // Value q alone, to or from its place.
     __device__ __forceinline__ void store_one(char* p, int q) const {
         if constexpr (ES == 4) *(word*)p = w[q];
         if constexpr (ES == 2) *(word2*)p = (unsigned short)(w[q / 2] >> (16 * (q & 1)));
-        if constexpr (ES == 1) *(unsigned char*)p = (unsigned char)(w[q / 4] >> (8 * (q & 3)));
+        if constexpr (ES == 1) *(unsigned char*)p = (unsigned char)(w[0] >> (8 * q));
     }
-    __device__ __forceinline__ void load_one(const char* p, int q) {   // q = 0, 1, ... in turn
+    __device__ __forceinline__ void load_one(const char* p, int q) {   // q = 0, 1, 2, 3 in turn
         if constexpr (ES == 4) w[q] = *(const word*)p;
         if constexpr (ES == 2) w[q / 2] = (q & 1 ? w[q / 2] : 0u) | (unsigned)*(const word2*)p << (16 * (q & 1));
-        if constexpr (ES == 1) w[q / 4] = (q & 3 ? w[q / 4] : 0u) | (unsigned)*(const unsigned char*)p << (8 * (q & 3));
+        if constexpr (ES == 1) w[0] = (q ? w[0] : 0u) | (unsigned)*(const unsigned char*)p << (8 * q);
     }
 
     // From values and their row's scale (NaN: zeros).
-    __device__ __forceinline__ void encode(const float (&x)[8], float s) {
+    __device__ __forceinline__ void encode(const float (&x)[4], float s) {
         const bool bad = s != s;
         if constexpr (ES > 1) {
             // s is a power of two, 2^-126 .. 2^113; a product with 1/s would lose -0 in its conversion to
             // halves (one instruction that adds +0)
             const int up = 127 - (int)(__float_as_uint(s) >> 23);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
+            for (int k = 0; k < 4; ++k) {
                 const float y = bad ? 0.f : __builtin_amdgcn_ldexpf(x[k], up);
                 if constexpr (ES == 4) {
                     w[k] = __float_as_uint(y);
@@ -107,129 +107,162 @@ struct alignas(cache_elem(TYPE) == 1 ? 8 : 16) Chunk {
                 }
             }
         } else {
+            // The quotient lies between x·lo and x·hi; where both round to the same stored values, those are
+            // its roundings.  The others, a few in a million and exact ties, are divided.
+            const float inv = bad ? 0.f : 1.f / s, lo = inv * (1.f - 0x1p-21f), hi = inv * (1.f + 0x1p-21f);
+            if constexpr (TYPE == LBR_CACHE_I8) {
+                unsigned u[4], far = 0;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
+                for (int k = 0; k < 4; ++k) {   // 1.5·2^23 + n holds n in its low bits, rounded once
+                    u[k] = __float_as_uint(fmaf(bad ? 0.f : x[k], hi, 0x1.8p23f));
+                    far |= u[k] ^ __float_as_uint(fmaf(bad ? 0.f : x[k], lo, 0x1.8p23f));
+                }
+                if (far) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) u[k] = (unsigned)(int)rintf(quotient_odd(x[k], s));
+                }
+                w[0] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(u[3], u[2], 0x0c0c0400u),
+                                             __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), 0x05040100u);
+            } else {
+                auto pack = [](float y0, float y1, float y2, float y3) {
+                    const int half = __builtin_amdgcn_cvt_pk_fp8_f32(y0, y1, 0, false);
+                    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(y2, y3, half, true);
+                };
                 float y[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) y[j] = bad ? 0.f : quotient_odd(x[4 * k + j], s);
-                if constexpr (TYPE == LBR_CACHE_I8) {
-                    w[k] = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) w[k] |= ((unsigned)(int)rintf(y[j]) & 255u) << (8 * j);
-                } else {
-                    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-                    w[k] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);
-                }
+                for (int k = 0; k < 4; ++k) y[k] = bad ? 0.f : x[k];
+                w[0] = pack(y[0] * hi, y[1] * hi, y[2] * hi, y[3] * hi);
+                if (w[0] != pack(y[0] * lo, y[1] * lo, y[2] * lo, y[3] * lo))
+                    w[0] = pack(quotient_odd(x[0], s), quotient_odd(x[1], s), quotient_odd(x[2], s), quotient_odd(x[3], s));
             }
         }
     }
-    // To values without their scale.
-    __device__ __forceinline__ void decode(float (&y)[8]) const {
+    // To values, times their row's scale.
+    __device__ __forceinline__ float4 decode(float s) const {
+        float y[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < 4; ++k) {
             if constexpr (ES == 4) y[k] = __uint_as_float(w[k]);
             if constexpr (ES == 2)
                 y[k] = (float)__builtin_bit_cast(_Float16, (unsigned short)(w[k / 2] >> (16 * (k & 1))));
-            if constexpr (TYPE == LBR_CACHE_I8) y[k] = (float)((int)(w[k / 4] << (24 - 8 * (k & 3))) >> 24);
+            if constexpr (TYPE == LBR_CACHE_I8) y[k] = (float)((int)(w[0] << (24 - 8 * k)) >> 24);
         }
         if constexpr (TYPE == LBR_CACHE_E4M3) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const floatx2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[k], false);
-                const floatx2 b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[k], true);
-                y[4 * k] = a[0]; y[4 * k + 1] = a[1]; y[4 * k + 2] = b[0]; y[4 * k + 3] = b[1];
-            }
+            const floatx2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[0], false);
+            const floatx2 b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[0], true);
+            y[0] = a[0];
+            y[1] = a[1];
+            y[2] = b[0];
+            y[3] = b[1];
         }
+        return make_float4(y[0] * s, y[1] * s, y[2] * s, y[3] * s);
     }
 };
 
-// Max over the eight lanes of a position.
-__device__ __forceinline__ unsigned max8(unsigned v) {
+// Max over aligned groups of G lanes.
+template <int G>
+__device__ __forceinline__ unsigned group_max(unsigned v) {
     v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false));    // lane ^ 1
     v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, false));    // lane ^ 2
-    return max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, false));   // 7 − lane
+    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, false));   // 7 − lane of 8
+    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, false));   // 15 − lane of 16
+    if (G >= 32) {
+        auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = max((unsigned)a[0], (unsigned)a[1]);
+    }
+    if (G == 64) {
+        auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = max((unsigned)a[0], (unsigned)a[1]);
+    }
+    return v;
+}
+
+// Four columns of a row of the fp32 tensors, zeros where there are none.
+__device__ __forceinline__ void load4(const float* p, int col, int hd, bool vec, float (&x)[4]) {
+    if (vec && col < hd) {   // hd is a multiple of four
+        const float4 v = *(const float4*)(p + col);
+        x[0] = v.x;
+        x[1] = v.y;
+        x[2] = v.z;
+        x[3] = v.w;
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[q] = col + q < hd ? p[col + q] : 0.f;
+    }
+}
+__device__ __forceinline__ void store4(float* p, int col, int hd, bool vec, float4 v) {
+    if (vec && col < hd) {
+        *(float4*)(p + col) = v;
+    } else {
+        const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (col + q < hd) p[col + q] = x[q];
+    }
 }
 
 // ---------------------------------------------------------------- the write
 
-// Unit of a wavefront: (b, h, g), V group start[b]/8 + g of the sequence.  NCH: chunks of 8 columns a lane.
-template <int TYPE, int NCH>
+// Unit of a wavefront: (b, h, g), V group start[b]/8 + g of the sequence.  LPR: lanes of a row (head_dim / 4, to 16,
+// 32 or 64); pass j takes positions j·64/LPR .. of the group.
+template <int TYPE, int LPR>
 __global__ __launch_bounds__(256) void cache_write(PagedCache c, const float* __restrict__ k,
                                                    const float* __restrict__ v, int S, int groups, unsigned units,
                                                    bool vec) {
-    constexpr int ES = cache_elem(TYPE);
-    __shared__ __attribute__((aligned(16))) char stage[4][64 * NCH * 8 * ES];
+    constexpr int ES = cache_elem(TYPE), RP = 64 / LPR, NP = 8 / RP;
+    __shared__ __attribute__((aligned(16))) char stage[4][4 * LPR * 8 * ES];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const unsigned unit = blockIdx.x * 4u + wave;
     if (unit >= units) return;   // whole wavefronts; no barrier below
     const int g = unit % groups, bh = unit / groups;
     const int h = bh % c.heads, b = bh / c.heads;
     const int start = c.start[b], count = min(max(c.count[b], 0), S);
-    const int r = lane >> 3, cl = lane & 7;
     const long long group = (start >> 3) + g;           // of eight positions
-    const long long row = group * 8 + r - start;        // of the chunk
-    const bool mine = row >= 0 && row < count;
-    if (!__any(mine)) return;
-    char* const head = cache_head(c, b, h, group * 8);   // a group never crosses a page
-    if (!head) return;
-    const int page_mask = (1 << c.shift) - 1;
-    const int slot = (int)(group * 8 + r) & page_mask;
-
-    const long long at = ((long long)bh * S + (mine ? row : 0)) * c.hd;
-    float xk[NCH][8], xv[NCH][8];
-    unsigned mk = 0, mv = 0;
+    const long long row0 = group * 8 - start;           // of the chunk, may lie before it
+    if (row0 + 8 <= 0 || row0 >= count) return;
+    const int col = lane % LPR * 4;
+    float xk[NP][4], xv[NP][4];
 #pragma unroll
-    for (int j = 0; j < NCH; ++j) {
-        const int col = (cl + 8 * j) * 8;
-        const bool whole = vec && col + 8 <= c.hd;
+    for (int j = 0; j < NP; ++j) {
+        const long long row = row0 + j * RP + lane / LPR;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) xk[j][q] = xv[j][q] = 0.f;
-        if (mine && whole) {
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const float4 a = *(const float4*)(k + at + col + 4 * q), e = *(const float4*)(v + at + col + 4 * q);
-                xk[j][4 * q] = a.x; xk[j][4 * q + 1] = a.y; xk[j][4 * q + 2] = a.z; xk[j][4 * q + 3] = a.w;
-                xv[j][4 * q] = e.x; xv[j][4 * q + 1] = e.y; xv[j][4 * q + 2] = e.z; xv[j][4 * q + 3] = e.w;
-            }
-        } else if (mine) {
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-                if (col + q < c.hd) {
-                    xk[j][q] = k[at + col + q];
-                    xv[j][q] = v[at + col + q];
-                }
+        for (int q = 0; q < 4; ++q) xk[j][q] = xv[j][q] = 0.f;
+        if (row >= 0 && row < count) {
+            const long long at = ((long long)bh * S + row) * c.hd;
+            load4(k + at, col, c.hd, vec, xk[j]);
+            load4(v + at, col, c.hd, vec, xv[j]);
         }
     }
+    char* const head = cache_head(c, b, h, group * 8);   // a group never crosses a page
+    if (!head) return;
+    const int page_mask = (1 << c.shift) - 1, slot0 = (int)(group * 8) & page_mask;
+    const bool full = row0 >= 0 && row0 + 8 <= count;    // else element by element
+    char* const vg = head + c.part + (long long)slot0 * c.hdp * ES;   // [hdp][8]
+    char* const st = stage[wave];
+    char* const to = full ? st : vg;
 #pragma unroll
-    for (int j = 0; j < NCH; ++j)
+    for (int j = 0; j < NP; ++j) {
+        const int r = j * RP + lane / LPR;
+        const long long row = row0 + r;
+        unsigned mk = 0, mv = 0;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
+        for (int q = 0; q < 4; ++q) {
             mk = max(mk, __float_as_uint(xk[j][q]) & 0x7fffffffu);
             mv = max(mv, __float_as_uint(xv[j][q]) & 0x7fffffffu);
         }
-    const float sk = row_scale<TYPE>(max8(mk)), sv = row_scale<TYPE>(max8(mv));
-    if (mine && cl == 0) {
-        float* sc = (float*)(head + 2 * c.part);
-        sc[slot] = sk;
-        sc[page_mask + 1 + slot] = sv;
-    }
-    // whole groups go through LDS, the rest element by element
-    const bool full = __all(mine);
-    char* const vg = head + c.part + (long long)(slot & ~7) * c.hdp * ES;   // [hdp][8]
-    char* const st = stage[wave];
-#pragma unroll
-    for (int j = 0; j < NCH; ++j) {
-        const int col = (cl + 8 * j) * 8;
-        if (col >= c.hdp) continue;
-        Chunk<TYPE> pk, pv;
+        const float sk = row_scale<TYPE>(group_max<LPR>(mk)), sv = row_scale<TYPE>(group_max<LPR>(mv));
+        if (row < 0 || row >= count || col >= c.hdp) continue;
+        if (col == 0) {
+            float* const sc = (float*)(head + 2 * c.part);
+            sc[slot0 + r] = sk;
+            sc[page_mask + 1 + slot0 + r] = sv;
+        }
+        Quad<TYPE> pk, pv;
         pk.encode(xk[j], sk);
         pv.encode(xv[j], sv);
-        if (mine) pk.store(head + ((long long)slot * c.hdp + col) * ES);
-        char* const to = full ? st : vg;
-        if (full || mine) {
+        pk.store(head + ((long long)(slot0 + r) * c.hdp + col) * ES);
 #pragma unroll
-            for (int q = 0; q < 8; ++q) pv.store_one(to + ((col + q) * 8 + r) * ES, q);
-        }
+        for (int q = 0; q < 4; ++q) pv.store_one(to + ((col + q) * 8 + r) * ES, q);
     }
     if (full) {
         __builtin_amdgcn_wave_barrier();
@@ -241,104 +274,92 @@ __global__ __launch_bounds__(256) void cache_write(PagedCache c, const float* __
 // ---------------------------------------------------------------- the read
 
 // Unit of a wavefront: (b, h, g) as in the write, for rows 0 .. T − 1 from position start[b].
-template <int TYPE, int NCH>
+template <int TYPE, int LPR>
 __global__ __launch_bounds__(256) void cache_read(PagedCache c, float* __restrict__ out, int B, int T, int groups,
                                                   unsigned units, bool vec) {
-    constexpr int ES = cache_elem(TYPE);
-    __shared__ __attribute__((aligned(16))) char stage[4][64 * NCH * 8 * ES];
+    constexpr int ES = cache_elem(TYPE), RP = 64 / LPR, NP = 8 / RP;
+    __shared__ __attribute__((aligned(16))) char stage[4][4 * LPR * 8 * ES];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const unsigned unit = blockIdx.x * 4u + wave;
     if (unit >= units) return;
     const int g = unit % groups, bh = unit / groups;
     const int h = bh % c.heads, b = bh / c.heads;
     const int start = c.start[b], count = min(max(c.count[b], 0), T);
-    const int r = lane >> 3, cl = lane & 7;
     const long long group = (start >> 3) + g;
-    const long long row = group * 8 + r - start;
-    const bool inside = row >= 0 && row < T;      // a row of the output
-    const bool mine = inside && row < count;      // that has a position
-    if (!__any(inside)) return;
-    const char* const head = __any(mine) ? cache_head(c, b, h, group * 8) : nullptr;
-    const int page_mask = (1 << c.shift) - 1;
-    const int slot = (int)(group * 8 + r) & page_mask;
+    const long long row0 = group * 8 - start;
+    if (row0 + 8 <= 0 || row0 >= T) return;
+    const bool some = row0 < count;                     // of the rows have a position
+    const char* const head = some ? cache_head(c, b, h, group * 8) : nullptr;
+    const int page_mask = (1 << c.shift) - 1, slot0 = (int)(group * 8) & page_mask;
+    const int col = lane % LPR * 4;
     const float nan = __uint_as_float(0x7fc00000u);
-    float sk = nan, sv = nan;
     char* const st = stage[wave];
+    Quad<TYPE> pk[NP];
+    float sk[NP], sv[NP];
     if (head) {
-        const float* sc = (const float*)(head + 2 * c.part);
-        sk = sc[slot];
-        sv = sc[page_mask + 1 + slot];
-        const char* const vg = head + c.part + (long long)(slot & ~7) * c.hdp * ES;
+        const char* const vg = head + c.part + (long long)slot0 * c.hdp * ES;
+        const float* const sc = (const float*)(head + 2 * c.part);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            const int r = j * RP + lane / LPR;
+            pk[j].load(head + ((long long)(slot0 + r) * c.hdp + (col < c.hdp ? col : 0)) * ES);
+            sk[j] = sc[slot0 + r];
+            sv[j] = sc[page_mask + 1 + slot0 + r];
+        }
         const int bytes = c.hdp * 8 * ES;
         for (int o = lane * 16; o < bytes; o += 1024) *(word16*)(st + o) = *(const word16*)(vg + o);
         __builtin_amdgcn_wave_barrier();
     }
     const long long half = (long long)B * c.heads * T * c.hd;   // K, then V
-    float* const ok = out + ((long long)bh * T + (inside ? row : 0)) * c.hd;
 #pragma unroll
-    for (int j = 0; j < NCH; ++j) {
-        const int col = (cl + 8 * j) * 8;
-        if (col >= c.hdp || !inside) continue;
-        float yk[8], yv[8];
+    for (int j = 0; j < NP; ++j) {
+        const int r = j * RP + lane / LPR;
+        const long long row = row0 + r;
+        if (row < 0 || row >= T || col >= c.hd) continue;
+        float4 yk = make_float4(0.f, 0.f, 0.f, 0.f), yv = yk;
+        if (row < count) {
+            yk = yv = make_float4(nan, nan, nan, nan);
+            if (head) {
+                Quad<TYPE> pv;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) yk[q] = yv[q] = mine ? nan : 0.f;
-        if (mine && head) {
-            Chunk<TYPE> pk, pv;
-            pk.load(head + ((long long)slot * c.hdp + col) * ES);
-#pragma unroll
-            for (int q = 0; q < 8; ++q) pv.load_one(st + ((col + q) * 8 + r) * ES, q);
-            pk.decode(yk);
-            pv.decode(yv);
-#pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                yk[q] *= sk;
-                yv[q] *= sv;
+                for (int q = 0; q < 4; ++q) pv.load_one(st + ((col + q) * 8 + r) * ES, q);
+                yk = pk[j].decode(sk[j]);
+                yv = pv.decode(sv[j]);
             }
         }
-        if (vec && col + 8 <= c.hd) {
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                *(float4*)(ok + col + 4 * q) = make_float4(yk[4 * q], yk[4 * q + 1], yk[4 * q + 2], yk[4 * q + 3]);
-                *(float4*)(ok + half + col + 4 * q) = make_float4(yv[4 * q], yv[4 * q + 1], yv[4 * q + 2], yv[4 * q + 3]);
-            }
-        } else {
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-                if (col + q < c.hd) {
-                    ok[col + q] = yk[q];
-                    ok[half + col + q] = yv[q];
-                }
-        }
+        float* const to = out + ((long long)bh * T + row) * c.hd;
+        store4(to, col, c.hd, vec, yk);
+        store4(to + half, col, c.hd, vec, yv);
     }
 }
 
 // ---------------------------------------------------------------- launchers
 
-template <int TYPE, int NCH>
+template <int TYPE, int LPR>
 void launch_write(const Step& s, hipStream_t st) {
     const int S = (int)s.i[7], groups = (int)((s.i[7] + 14) / 8);
     const long long units = s.i[1] * s.i[2] * groups;
     if (S <= 0 || units <= 0) return;
-    hipLaunchKernelGGL((cache_write<TYPE, NCH>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, paged_cache(s),
+    hipLaunchKernelGGL((cache_write<TYPE, LPR>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, paged_cache(s),
                        (const float*)s.in[4], (const float*)s.in[5], S, groups, (unsigned)units, s.i[9] != 0);
 }
 
-template <int TYPE, int NCH>
+template <int TYPE, int LPR>
 void launch_read(const Step& s, hipStream_t st) {
     const int T = (int)s.i[7], groups = (int)((s.i[7] + 14) / 8);
     const long long units = s.i[1] * s.i[2] * groups;
     if (T <= 0 || units <= 0) return;
-    hipLaunchKernelGGL((cache_read<TYPE, NCH>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, paged_cache(s),
+    hipLaunchKernelGGL((cache_read<TYPE, LPR>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, paged_cache(s),
                        (float*)s.out, (int)s.i[1], T, groups, (unsigned)units, s.i[9] != 0);
 }
 
 template <int TYPE>
 step_fn write_for(int hd) {
-    return hd <= 64 ? launch_write<TYPE, 1> : hd <= 128 ? launch_write<TYPE, 2> : launch_write<TYPE, 4>;
+    return hd <= 64 ? launch_write<TYPE, 16> : hd <= 128 ? launch_write<TYPE, 32> : launch_write<TYPE, 64>;
 }
 template <int TYPE>
 step_fn read_for(int hd) {
-    return hd <= 64 ? launch_read<TYPE, 1> : hd <= 128 ? launch_read<TYPE, 2> : launch_read<TYPE, 4>;
+    return hd <= 64 ? launch_read<TYPE, 16> : hd <= 128 ? launch_read<TYPE, 32> : launch_read<TYPE, 64>;
 }
 
 // Whether the wavefronts of a launch, one for each eight rows of a head, can be counted in its grid.
