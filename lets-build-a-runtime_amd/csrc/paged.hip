@@ -159,24 +159,6 @@ struct Quad {
     }
 };
 
-// Max over aligned groups of G lanes.
-template <int G>
-__device__ __forceinline__ unsigned group_max(unsigned v) {
-    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false));    // lane ^ 1
-    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, false));    // lane ^ 2
-    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, false));   // 7 − lane of 8
-    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, false));   // 15 − lane of 16
-    if (G >= 32) {
-        auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-        v = max((unsigned)a[0], (unsigned)a[1]);
-    }
-    if (G == 64) {
-        auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-        v = max((unsigned)a[0], (unsigned)a[1]);
-    }
-    return v;
-}
-
 // Four columns of a row of the fp32 tensors, zeros where there are none.
 __device__ __forceinline__ void load4(const float* p, int col, int hd, bool vec, float (&x)[4]) {
     if (vec && col < hd) {   // hd is a multiple of four
@@ -250,7 +232,7 @@ __global__ __launch_bounds__(256) void cache_write(PagedCache c, const float* __
             mk = max(mk, __float_as_uint(xk[j][q]) & 0x7fffffffu);
             mv = max(mv, __float_as_uint(xv[j][q]) & 0x7fffffffu);
         }
-        const float sk = row_scale<TYPE>(group_max<LPR>(mk)), sv = row_scale<TYPE>(group_max<LPR>(mv));
+        const float sk = row_scale<TYPE>(row_max_bits<LPR>(mk)), sv = row_scale<TYPE>(row_max_bits<LPR>(mv));
         if (row < 0 || row >= count || col >= c.hdp) continue;
         if (col == 0) {
             float* const sc = (float*)(head + 2 * c.part);

@@ -16,7 +16,7 @@
 
 #include "paged_common.h"
 
-// Launchers: rows of at most 64 a K/V head (paged_attention.hip), and more (paged_tiles.hip).
+// Launchers: rows of at most 32 a K/V head (paged_attention.hip), and more (paged_tiles.hip).
 step_fn paged_tiles_launcher(int type, int hd);
 // Ranges of the keys of paged_tiles (Step::i[10]), and its workspace.
 int paged_tiles_splits(const Step& s);
@@ -119,11 +119,14 @@ __device__ __forceinline__ float quad_sum(float v) {
     auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
-__device__ __forceinline__ unsigned quad_max_bits(unsigned v) {
-    auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    v = max((unsigned)a[0], (unsigned)a[1]);
-    auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return max((unsigned)b[0], (unsigned)b[1]);
+// Adds a partial result (a row's maximum, sum and weighted mean over some keys) to a running maximum, sum and
+// weighted sum.
+__device__ __forceinline__ void merge_part(float& m, float& l, floatx4& o, float pm, float pl, floatx4 mean) {
+    const float mx = fmaxf(m, pm), base = mx == -INFINITY ? 0.f : mx;
+    const float f = __builtin_amdgcn_exp2f(m - base), g = __builtin_amdgcn_exp2f(pm - base) * pl;
+    o = o * f + mean * g;
+    l = l * f + g;
+    m = mx;
 }
 
 // Biased exponent of the power of two that brings a magnitude's bits into [2^14, 2^15), at most 2^127.

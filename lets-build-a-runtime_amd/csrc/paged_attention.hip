@@ -5,7 +5,7 @@ namespace {
 
 // ---------------------------------------------------------------- few rows: split over the keys
 //
-// At most 64 rows a K/V head (single tokens, drafted tokens): the cache is read once and bounds the time.  A
+// At most 32 rows a K/V head (single tokens, drafted tokens): the cache is read once and bounds the time.  A
 // step is 32 keys of one wavefront, 128 of a workgroup; the steps of all (sequence, K/V head) segments lie in
 // one line, which the workgroups cut into equal ranges, so that a batch of one long and many short
 // sequences fills the chip as an even one does.  A segment inside one range is finished there; one that ranges cut
@@ -20,55 +20,65 @@ namespace {
 
 constexpr int STEP = 32, WAVES = 4, STEP_WG = STEP * WAVES;
 
-// Steps of a workgroup (128 keys) that sequence b takes, at least one: its rows are written in any case.
-__device__ __forceinline__ int steps_of(const PagedAttn& a, int b) {
-    return max(1, (span_of(a, b).keys + STEP_WG - 1) / STEP_WG);
-}
+// Steps of a workgroup (128 keys) that a sequence takes, at least one: its rows are written in any case.
+__device__ __forceinline__ int steps_of(const Span& s) { return max(1, (s.keys + STEP_WG - 1) / STEP_WG); }
 
-// Where the ranges lie: sums of steps before each of 256 blocks of sequences (LDS), and the whole.
+// The line, 64 sequences at a time: lane b holds sequence first + b and the inclusive sum of steps up to it, both
+// of one K/V head.  Every wavefront builds it for itself, without a barrier.
 struct Line {
-    long long before[257];
+    Span sp;
+    int first, steps, run;
+    long long before;   // steps of the sequences before `first`
 };
 
-__device__ __forceinline__ void line_build(const PagedAttn& a, Line& ln) {
-    __shared__ long long wave_sum[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = (a.B + 255) / 256;
-    long long mine = 0;
-    for (int b = tid * per; b < min((tid + 1) * per, a.B); ++b) mine += steps_of(a, b);
-    long long run = mine;
+__device__ __forceinline__ void line_load(const PagedAttn& a, Line& ln) {
+    const int lane = threadIdx.x & 63, b = ln.first + lane;
+    ln.sp = span_of(a, min(b, a.B - 1));
+    ln.steps = b < a.B ? steps_of(ln.sp) : 0;
+    ln.run = ln.steps;
     for (int o = 1; o < 64; o <<= 1) {
-        const long long t = __shfl_up(run, o, 64);
-        if (lane >= o) run += t;
+        const int t = __shfl_up(ln.run, o, 64);
+        if (lane >= o) ln.run += t;
     }
-    if (lane == 63) wave_sum[wave] = run;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) run += wave_sum[w];
-    ln.before[tid + 1] = run;
-    if (tid == 0) ln.before[0] = 0;
-    __syncthreads();
+}
+// From the first sequence on, and all steps of a head.
+__device__ __forceinline__ long long line_begin(const PagedAttn& a, Line& ln) {
+    long long all = 0;
+    for (int first = (a.B - 1) / 64 * 64; first >= 0; first -= 64) {
+        ln.first = first;
+        line_load(a, ln);
+        all += __builtin_amdgcn_readlane(ln.run, 63);
+    }
+    ln.before = 0;
+    return all;
+}
+__device__ __forceinline__ void line_next(const PagedAttn& a, Line& ln) {
+    ln.before += __builtin_amdgcn_readlane(ln.run, 63);
+    ln.first += 64;
+    line_load(a, ln);
 }
 
-// Sequence that step x (of one head's worth of steps a sequence, all heads: x / heads) falls to, and the steps before it.
-__device__ __forceinline__ void line_find(const PagedAttn& a, const Line& ln, long long x, int& b, long long& before) {
-    __shared__ int found_b;
-    __shared__ long long found_before;
-    const int tid = threadIdx.x, per = (a.B + 255) / 256;
+// A sequence of the line: itself, its span and steps, and the steps before it.
+struct Place {
+    int b, steps;
+    Span sp;
+    long long before;
+};
+__device__ __forceinline__ Place line_place(const Line& ln, int lane) {
+    Place p;
+    p.b = ln.first + lane;
+    p.steps = __builtin_amdgcn_readlane(ln.steps, lane);
+    p.sp.start = __builtin_amdgcn_readlane(ln.sp.start, lane);
+    p.sp.count = __builtin_amdgcn_readlane(ln.sp.count, lane);
+    p.sp.keys = __builtin_amdgcn_readlane(ln.sp.keys, lane);
+    p.before = ln.before + __builtin_amdgcn_readlane(ln.run, lane) - p.steps;
+    return p;
+}
+// The sequence that step x of all heads' falls to; x lies in the line.
+__device__ __forceinline__ Place line_seek(const PagedAttn& a, Line& ln, long long x) {
     const long long heads = a.c.heads;
-    if (x >= ln.before[tid] * heads && x < ln.before[tid + 1] * heads) {
-        long long at = ln.before[tid];
-        int k = tid * per;
-        for (;; ++k) {
-            const int n = steps_of(a, k);
-            if (x < (at + n) * heads) break;
-            at += n;
-        }
-        found_b = k;
-        found_before = at;
-    }
-    __syncthreads();
-    b = found_b;
-    before = found_before;
+    while (x >= (ln.before + __builtin_amdgcn_readlane(ln.run, 63)) * heads) line_next(a, ln);
+    return line_place(ln, __builtin_ctzll(__ballot(x < (ln.before + ln.run) * heads)));
 }
 
 // Range w of W ≤ T over T steps starts at w·T/W; the range that step x falls to.
@@ -79,14 +89,29 @@ __device__ __forceinline__ long long range_of(long long x, long long W, long lon
 template <int HD, int NR>
 constexpr int part_floats() { return 16 * NR * (HD + 2); }
 
+// A wavefront's registers, about: tiles in flight, accumulators, the rest.  Two workgroups a CU where 256 registers
+// are enough, with two tiles or else one; otherwise one, with two tiles where they fit.  (32 sequences, float16: two
+// workgroups of one tile 63 µs, one of two 80.)
 template <int TYPE, int HD, int NR>
-__global__ __launch_bounds__(256, 2) void paged_split(PagedAttn a) {
+constexpr int split_registers(int tiles) {
+    return tiles * (HD * cache_elem(TYPE) / 4 + 16) + NR * HD / 4 + 64 + 16 * NR;
+}
+template <int TYPE, int HD, int NR>
+constexpr int split_occupancy() { return split_registers<TYPE, HD, NR>(1) <= 256 ? 2 : 1; }
+template <int TYPE, int HD, int NR>
+constexpr int split_tiles() { return split_registers<TYPE, HD, NR>(2) <= (split_occupancy<TYPE, HD, NR>() == 2 ? 256 : 480) ? 2 : 1; }
+
+template <int TYPE, int HD, int NR>
+__global__ __launch_bounds__(256, (split_occupancy<TYPE, HD, NR>())) void paged_split(PagedAttn a) {
     constexpr int ES = cache_elem(TYPE);
     constexpr int NK = HD / 32;          // MFMA steps over the columns
     constexpr int ND = HD / 16;          // 16-column blocks of the output
     constexpr int PL = TYPE == LBR_CACHE_F32 ? 2 : 1;
     constexpr int ROWS = 16 * NR;
-    __shared__ Line line;
+    constexpr bool TWO = split_tiles<TYPE, HD, NR>() == 2;
+    constexpr int LPR = HD / 4;          // threads of a row where all load or store it
+    __shared__ __attribute__((aligned(16))) _Float16 q_lds[2 * NR * NK * 512];   // [16 rows][MFMA step][h, l][lane][8]
+    __shared__ float q_scale[ROWS];
     __shared__ float wave_m[WAVES][ROWS], wave_l[WAVES][ROWS];
     __shared__ int wave_up[WAVES];
     __shared__ __attribute__((aligned(16))) float hand[2][ROWS * HD];
@@ -96,17 +121,14 @@ __global__ __launch_bounds__(256, 2) void paged_split(PagedAttn a) {
     const PagedCache& c = a.c;
     const int page = 1 << c.shift, mask = page - 1;
 
-    line_build(a, line);
-    const long long T = line.before[256] * c.heads, W = min((long long)gridDim.x, T), w = blockIdx.x;
+    Line line;
+    const long long T = line_begin(a, line) * c.heads, W = min((long long)gridDim.x, T), w = blockIdx.x;
     if (w >= W) return;
     long long x = range_start(w, W, T);
     const long long first = x, end = range_start(w + 1, W, T);
-    int b;
-    long long before;
-    line_find(a, line, x, b, before);
-    int steps = steps_of(a, b);
-    int h = (int)((x - before * c.heads) / steps);
-    int at = (int)(x - before * c.heads - (long long)h * steps);
+    Place pl = line_seek(a, line, x);
+    int h = (int)((x - pl.before * c.heads) / pl.steps);
+    int at = (int)(x - pl.before * c.heads - (long long)h * pl.steps);
 
     // columns of a lane's loads, clamped to the row (q is zero behind it)
     int koff[NK], voff[ND];
@@ -121,54 +143,140 @@ __global__ __launch_bounds__(256, 2) void paged_split(PagedAttn a) {
         voff[j] = (col < c.hdp ? col : 0) * 8 * ES;
     }
 
-    while (x < end) {   // segments
-        const Span sp = span_of(a, b);
-        const int stop = (int)min((long long)steps, at + (end - x));   // steps at .. stop − 1 of this segment
+    // a wavefront's 32 keys of a step, as loaded
+    struct Tile {
+        uint4 k[2][NK * ES / 2], v[ND * ES / 2];
+        float ks[8], vs[8];
+    };
+    struct Pages {
+        int lo, hi;   // of its first and its last 16 keys
+    };
 
-        // rows of q: two halves, scaled; row 16·t + n
-        halfx8 qh[NR][NK], ql[NR][NK];
-        float qs[NR];
-        int last[NR];   // last key of the row
+    while (x < end) {   // segments
+        const Span sp = pl.sp;
+        const int b = pl.b, steps = pl.steps;
+        const int stop = (int)min((long long)steps, at + (end - x));   // steps at .. stop − 1 of this segment
+        // the wavefront's own: those that begin before the end
+        const int mine = min(stop, (sp.keys - wave * STEP + STEP_WG - 1) / STEP_WG);
+        const int lastg = (sp.keys - 1) & ~7;
+        // Read through the scalar cache: in the order of vector loads a wait for them would be one for the tile
+        // behind them.
+        typedef const __attribute__((address_space(4))) int* Table;
+        const Table tab = (Table)(c.table + (long long)b * c.wide);
+        auto pages = [&](int st) {
+            const int k0 = st * STEP_WG + wave * STEP;
+            return Pages{tab[min(k0, lastg) >> c.shift], tab[min(k0 + 16, lastg) >> c.shift]};
+        };
+        auto is_page = [&](int p) { return p >= 0 && p < c.pages; };
+        auto load = [&](Tile& t, int st, Pages p) {
+            // the groups of eight keys that a lane loads K rows (n / 4) and V columns (kg) of, clamped to the last
+            const int k0 = st * STEP_WG + wave * STEP;
+            const int gk = min(k0 + 8 * (n >> 2), lastg), gv = min(k0 + 8 * kg, lastg);
+            const char* const lo = c.base + (is_page(p.lo) ? p.lo : 0) * c.page_bytes + (long long)h * c.head_bytes;
+            const char* const hi = c.base + (is_page(p.hi) ? p.hi : 0) * c.page_bytes + (long long)h * c.head_bytes;
+            const char* const hk = n >= 8 ? hi : lo;
+            const char* const hv = kg >= 2 ? hi : lo;
 #pragma unroll
-        for (int t = 0; t < NR; ++t) {
-            const int r = 16 * t + n;
-            const int token = (int)lbr_fdiv((unsigned)min(r, a.rows - 1), a.G_m, a.G_s), g = min(r, a.rows - 1) - token * a.G;
-            const float* const qr = a.q + ((long long)(b * a.H + h * a.G + g) * a.S + token) * c.hd;
-            last[t] = r < a.rows && token < sp.count ? sp.start + token : -1;
-            float v[NK][8];
-            unsigned top = 0;
+            for (int u = 0; u < 2; ++u) {
+                const char* const row = hk + ((gk & mask) + 4 * u + (n & 3)) * c.hdp * ES;
 #pragma unroll
-            for (int j = 0; j < NK; ++j) {
-                const int col = ES == 1 ? (j / 2) * 64 + kg * 16 + (j % 2) * 8 : j * 32 + kg * 8;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) v[j][k] = 0.f;
-                if (last[t] >= 0) {
-                    if (a.vec && col + 8 <= c.hd) {
-                        const float4 u0 = *(const float4*)(qr + col), u1 = *(const float4*)(qr + col + 4);
-                        v[j][0] = u0.x; v[j][1] = u0.y; v[j][2] = u0.z; v[j][3] = u0.w;
-                        v[j][4] = u1.x; v[j][5] = u1.y; v[j][6] = u1.z; v[j][7] = u1.w;
+                for (int j = 0; j < NK; ++j) {
+                    if (ES == 1) {
+                        if (j % 2 == 0) t.k[u][j / 2] = *(const uint4*)(row + koff[j]);
                     } else {
 #pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            if (col + k < c.hd) v[j][k] = qr[col + k];
+                        for (int e = 0; e < ES / 2; ++e) t.k[u][j * (ES / 2) + e] = *(const uint4*)(row + koff[j] + 16 * e);
                     }
                 }
+            }
+            const float* const sc = (const float*)(hv + 2 * c.part) + (gv & mask);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    v[j][k] *= a.scale;
-                    top = max(top, __float_as_uint(v[j][k]) & 0x7fffffffu);
+            for (int e = 0; e < 2; ++e) {
+                const float4 u = *(const float4*)(sc + 4 * e), v = *(const float4*)(sc + page + 4 * e);
+                t.ks[4 * e] = u.x; t.ks[4 * e + 1] = u.y; t.ks[4 * e + 2] = u.z; t.ks[4 * e + 3] = u.w;
+                t.vs[4 * e] = v.x; t.vs[4 * e + 1] = v.y; t.vs[4 * e + 2] = v.z; t.vs[4 * e + 3] = v.w;
+            }
+            const char* const vb = hv + c.part + (gv & mask) * c.hdp * ES;
+#pragma unroll
+            for (int j = 0; j < ND; ++j) {
+                if (ES == 1) {
+                    if (j % 2 == 0) t.v[j / 2] = *(const uint4*)(vb + voff[j]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < ES / 2; ++e) t.v[j * (ES / 2) + e] = *(const uint4*)(vb + voff[j] + 16 * e);
                 }
             }
-            top = quad_max_bits(top);
-            const int up = up_exponent(top);
-            const float by = __uint_as_float((unsigned)up << 23);
-            qs[t] = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float((unsigned)(254 - up) << 23);
+        };
+        Tile ta, tb;
+        Pages here = {0, 0}, next = {0, 0};   // of the step being computed, and of the next
+        if (at < mine) {
+            here = pages(at);
+            if (at + 1 < mine) next = pages(at + 1);
+            load(ta, at, here);
+        }
+
+        // rows of q into LDS: two halves, scaled, in the order of the MFMAs' operands
+        int hd = c.hd;
+        asm volatile("" : "+s"(hd));   // or what depends on it alone is worked out ahead of the loop, and spilled
+        {
+            const int col = tid % LPR * 4;
+            const int j = ES == 1 ? col / 64 * 2 + col % 16 / 8 : col / 32, g4 = ES == 1 ? col % 64 / 16 : col % 32 / 8;
+            constexpr int EACH = ROWS * LPR / 256;   // rows a thread
+            float v[EACH][4];
 #pragma unroll
-            for (int j = 0; j < NK; ++j) {
+            for (int i = 0; i < EACH; ++i) {   // all loads go out together
+                const int r = i * (256 / LPR) + tid / LPR;
+                const int token = (int)lbr_fdiv((unsigned)min(r, a.rows - 1), a.G_m, a.G_s), g = min(r, a.rows - 1) - token * a.G;
+                const float* const qr = a.q + ((long long)(b * a.H + h * a.G + g) * a.S + token) * hd;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[j][k] *= by;
-                split8(v[j], qh[t][j], ql[t][j]);
+                for (int k = 0; k < 4; ++k) v[i][k] = 0.f;
+                if (r < a.rows && token < sp.count) {
+                    if (a.vec && col < hd) {
+                        const float4 u = *(const float4*)(qr + col);
+                        v[i][0] = u.x;
+                        v[i][1] = u.y;
+                        v[i][2] = u.z;
+                        v[i][3] = u.w;
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (col + k < hd) v[i][k] = qr[col + k];
+                    }
+                }
             }
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const int r = i * (256 / LPR) + tid / LPR;
+                unsigned top = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    v[i][k] *= a.scale;
+                    top = max(top, __float_as_uint(v[i][k]) & 0x7fffffffu);
+                }
+                top = row_max_bits<LPR>(top);
+                const int up = up_exponent(top);
+                const float by = __uint_as_float((unsigned)up << 23);
+                halfx4 hi, lo;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    hi[k] = (_Float16)(v[i][k] * by);
+                    lo[k] = (_Float16)(v[i][k] * by - (float)hi[k]);
+                }
+                _Float16* const to = q_lds + ((r / 16 * NK + j) * 2 * 64 + g4 * 16 + r % 16) * 8 + col % 8;
+                *(halfx4*)to = hi;
+                *(halfx4*)(to + 512) = lo;
+                if (col == 0)
+                    q_scale[r] = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float((unsigned)(254 - up) << 23);
+            }
+        }
+        __syncthreads();
+        float qs[NR];
+        int last[NR];   // last key of row 16·t + n
+#pragma unroll
+        for (int t = 0; t < NR; ++t) {
+            const int r = 16 * t + n, token = (int)lbr_fdiv((unsigned)min(r, a.rows - 1), a.G_m, a.G_s);
+            qs[t] = q_scale[r];
+            last[t] = r < a.rows && token < sp.count ? sp.start + token : -1;
         }
 
         floatx4 o[NR][ND];
@@ -182,112 +290,102 @@ __global__ __launch_bounds__(256, 2) void paged_split(PagedAttn a) {
             for (int j = 0; j < ND; ++j) o[t][j] = floatx4{0.f, 0.f, 0.f, 0.f};
         }
 
-        for (int st = at; st < stop; ++st) {
+        auto compute = [&](Tile& t, int st, Pages at_page) {
             const int k0 = st * STEP_WG + wave * STEP;
-            if (k0 >= sp.keys) break;   // wave-uniform
-            // the groups of eight keys that this lane loads K rows (n / 4) and V columns (kg) of, clamped to the last
-            const int lastg = (sp.keys - 1) & ~7;
-            const int gk = min(k0 + 8 * (n >> 2), lastg), gv = min(k0 + 8 * kg, lastg);
-            const int* const tab = c.table + (long long)b * c.wide;
-            const int pk = tab[gk >> c.shift], pv = tab[gv >> c.shift];
-            const bool badv = pv < 0 || pv >= c.pages;
-            const char* const hk = c.base + (pk < 0 || pk >= c.pages ? 0 : pk) * c.page_bytes + (long long)h * c.head_bytes;
-            const char* const hv = c.base + (badv ? 0 : pv) * c.page_bytes + (long long)h * c.head_bytes;
-
-            uint4 kr[2][NK * ES / 2], vr[ND * ES / 2];
+            // keys behind the end, and pages that are none, hold anything
+            const bool badv = !is_page(kg >= 2 ? at_page.hi : at_page.lo);
+            const int keep = sp.keys - (k0 + 8 * kg);   // of the lane's eight keys
+            const bool tail = k0 + STEP > sp.keys;
+            if (tail || !is_page(at_page.lo) || !is_page(at_page.hi)) {
+                const int keepv = badv ? 0 : keep;
+                unsigned to[4];   // words of eight values, as far as the type has them
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const char* const row = hk + (long long)((gk & mask) + 4 * t + (n & 3)) * c.hdp * ES;
+                for (int e = 0; e < 4; ++e) {
+                    const int bits = ES == 1 ? 8 * min(max(keepv - 4 * (e & 1), 0), 4) : 16 * min(max(keepv - 2 * e, 0), 2);
+                    to[e] = bits == 32 ? ~0u : (1u << bits) - 1u;
+                }
 #pragma unroll
-                for (int j = 0; j < NK; ++j) {
-                    if (ES == 1) {
-                        if (j % 2 == 0) kr[t][j / 2] = *(const uint4*)(row + koff[j]);
+                for (int j = 0; j < ND * ES / 2; ++j) {
+                    if (ES == 4) {
+                        const int e = j % 2 * 4;
+                        t.v[j].x = e < keepv ? t.v[j].x : 0u;
+                        t.v[j].y = e + 1 < keepv ? t.v[j].y : 0u;
+                        t.v[j].z = e + 2 < keepv ? t.v[j].z : 0u;
+                        t.v[j].w = e + 3 < keepv ? t.v[j].w : 0u;
                     } else {
-#pragma unroll
-                        for (int e = 0; e < ES / 2; ++e) kr[t][j * (ES / 2) + e] = *(const uint4*)(row + koff[j] + 16 * e);
+                        t.v[j].x &= to[0];
+                        t.v[j].y &= to[1];
+                        t.v[j].z &= to[2];
+                        t.v[j].w &= to[3];
                     }
                 }
-            }
-            const char* const vb = hv + c.part + (long long)(gv & mask) * c.hdp * ES;
 #pragma unroll
-            for (int j = 0; j < ND; ++j) {
-                if (ES == 1) {
-                    if (j % 2 == 0) vr[j / 2] = *(const uint4*)(vb + voff[j]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < ES / 2; ++e) vr[j * (ES / 2) + e] = *(const uint4*)(vb + voff[j] + 16 * e);
+                for (int e = 0; e < 8; ++e) {
+                    if (badv) t.ks[e] = t.vs[e] = __uint_as_float(0x7fc00000u);
+                    if (e >= keep) t.vs[e] = 0.f;
                 }
-            }
-            float ks[8], vs[8];
-            {
-                const float* const sc = (const float*)(hv + 2 * c.part) + (gv & mask);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float4 u = *(const float4*)(sc + 4 * e), v = *(const float4*)(sc + page + 4 * e);
-                    ks[4 * e] = u.x; ks[4 * e + 1] = u.y; ks[4 * e + 2] = u.z; ks[4 * e + 3] = u.w;
-                    vs[4 * e] = v.x; vs[4 * e + 1] = v.y; vs[4 * e + 2] = v.z; vs[4 * e + 3] = v.w;
-                }
-            }
-            // keys behind the end, and pages that are none
-            const bool tail = k0 + STEP > sp.keys;
-            const int keep = sp.keys - (k0 + 8 * kg);   // of the lane's eight keys
-            const int keepv = badv ? 0 : keep;
-            const bool cut = tail || __any(badv);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if (badv) ks[e] = vs[e] = __uint_as_float(0x7fc00000u);
-                if (tail && e >= keep) vs[e] = 0.f;
             }
 
             // scores, two blocks of 16 keys
             floatx4 s[NR][2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int r = 0; r < NR; ++r) s[r][0] = s[r][1] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int r = 0; r < NR; ++r) s[r][t] = floatx4{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < NK; ++j) {
+                halfx8 kh[2], kl[2];
 #pragma unroll
-                for (int j = 0; j < NK; ++j) {
-                    halfx8 kh, kl;
+                for (int u = 0; u < 2; ++u) {
                     if constexpr (TYPE == LBR_CACHE_F32) {
-                        const uint4 u = kr[t][2 * j], v = kr[t][2 * j + 1];
-                        const float f[8] = {__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w),
-                                            __uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
-                        split8(f, kh, kl);
+                        const uint4 y = t.k[u][2 * j], z = t.k[u][2 * j + 1];
+                        const float f[8] = {__uint_as_float(y.x), __uint_as_float(y.y), __uint_as_float(y.z), __uint_as_float(y.w),
+                                            __uint_as_float(z.x), __uint_as_float(z.y), __uint_as_float(z.z), __uint_as_float(z.w)};
+                        split8(f, kh[u], kl[u]);
                     } else if constexpr (TYPE == LBR_CACHE_F16) {
-                        kh = __builtin_bit_cast(halfx8, kr[t][j]);
+                        kh[u] = __builtin_bit_cast(halfx8, t.k[u][j]);
                     } else {
-                        const uint4 u = kr[t][j / 2];
-                        kh = j % 2 ? widen8<TYPE>(u.z, u.w) : widen8<TYPE>(u.x, u.y);
+                        const uint4 y = t.k[u][j / 2];
+                        kh[u] = j % 2 ? widen8<TYPE>(y.z, y.w) : widen8<TYPE>(y.x, y.y);
                     }
+                }
 #pragma unroll
-                    for (int r = 0; r < NR; ++r) {
-                        s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[r][j], s[r][t], 0, 0, 0);
-                        if constexpr (PL == 2) s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[r][j], s[r][t], 0, 0, 0);
-                        s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[r][j], s[r][t], 0, 0, 0);
+                for (int r = 0; r < NR; ++r) {
+                    const halfx8 hi = *(const halfx8*)(q_lds + ((r * NK + j) * 2 * 64 + lane) * 8);
+                    const halfx8 lo = *(const halfx8*)(q_lds + ((r * NK + j) * 2 * 64 + 64 + lane) * 8);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        s[r][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[u], lo, s[r][u], 0, 0, 0);
+                        if constexpr (PL == 2) s[r][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[u], hi, s[r][u], 0, 0, 0);
+                        s[r][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[u], hi, s[r][u], 0, 0, 0);
                     }
                 }
             }
 
+            __builtin_amdgcn_sched_barrier(0);   // or values widened ahead of their phase spill
             // the V rows' scales over a running power of two
             float vtop = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) vtop = fmaxf(vtop, vs[e]);
+            for (int e = 0; e < 8; ++e) vtop = fmaxf(vtop, t.vs[e]);
             vtop = quad_max(vtop);
             const int vnew = __builtin_amdgcn_readfirstlane(min(vup, up_exponent(__float_as_uint(vtop))));
             const float vby = __uint_as_float((unsigned)vnew << 23);
+            float vs[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) vs[e] *= vby;
+            for (int e = 0; e < 8; ++e) vs[e] = t.vs[e] * vby;
 
+            const bool edge = tail || k0 + STEP - 1 > sp.start;   // some row ends among these keys
             halfx8 ph[NR], pl[NR];
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
                 float sc[8], top = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    sc[e] = s[r][e >> 2][e & 3] * (ks[e] * qs[r]);
-                    if (k0 + 8 * kg + e > last[r] || (tail && e >= keep)) sc[e] = -INFINITY;
-                    top = fmaxf(top, sc[e]);
+                for (int e = 0; e < 8; ++e) sc[e] = s[r][e >> 2][e & 3] * (t.ks[e] * qs[r]);
+                if (edge) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (k0 + 8 * kg + e > last[r]) sc[e] = -INFINITY;   // a row's last key lies before the end
                 }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, sc[e]);
                 const float mx = fmaxf(m[r], quad_max(top));
                 const float base = mx == -INFINITY ? 0.f : mx;
                 const float alpha = __builtin_amdgcn_exp2f(m[r] - base);
@@ -297,39 +395,35 @@ __global__ __launch_bounds__(256, 2) void paged_split(PagedAttn a) {
                 for (int e = 0; e < 8; ++e) {
                     p[e] = __builtin_amdgcn_exp2f(sc[e] - base);
                     sum += p[e];
-                    p[e] = sc[e] == -INFINITY ? 0.f : p[e] * vs[e];   // no weight, whatever the V row holds
+                    p[e] *= vs[e];
+                }
+                if (edge) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (sc[e] == -INFINITY) p[e] = 0.f;   // no weight, whatever the V row holds
                 }
                 l[r] = l[r] * alpha + sum;
                 split8(p, ph[r], pl[r]);
                 const float f = __builtin_amdgcn_ldexpf(alpha, vnew - vup);
-                if (__any(f != 1.f)) {
-                    asm volatile("");   // a branch: done ahead of it, the products would need registers of their own
 #pragma unroll
-                    for (int j = 0; j < ND; ++j) o[r][j] *= f;
-                }
+                for (int j = 0; j < ND; ++j) o[r][j] *= f;
             }
             vup = vnew;
+            __builtin_amdgcn_sched_barrier(0);
 
 #pragma unroll
             for (int j = 0; j < ND; ++j) {
                 halfx8 vh, vl;
                 if constexpr (TYPE == LBR_CACHE_F32) {
-                    const uint4 u = vr[2 * j], v = vr[2 * j + 1];
-                    const float f[8] = {__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w),
-                                        __uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
+                    const uint4 y = t.v[2 * j], z = t.v[2 * j + 1];
+                    const float f[8] = {__uint_as_float(y.x), __uint_as_float(y.y), __uint_as_float(y.z), __uint_as_float(y.w),
+                                        __uint_as_float(z.x), __uint_as_float(z.y), __uint_as_float(z.z), __uint_as_float(z.w)};
                     split8(f, vh, vl);
                 } else if constexpr (TYPE == LBR_CACHE_F16) {
-                    vh = __builtin_bit_cast(halfx8, vr[j]);
+                    vh = __builtin_bit_cast(halfx8, t.v[j]);
                 } else {
-                    const uint4 u = vr[j / 2];
-                    vh = j % 2 ? widen8<TYPE>(u.z, u.w) : widen8<TYPE>(u.x, u.y);
-                }
-                if (cut) {   // what lies behind the end may be anything
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        if (e >= keepv) vh[e] = (_Float16)0.f;
-                        if (PL == 2 && e >= keepv) vl[e] = (_Float16)0.f;
-                    }
+                    const uint4 y = t.v[j / 2];
+                    vh = j % 2 ? widen8<TYPE>(y.z, y.w) : widen8<TYPE>(y.x, y.y);
                 }
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
@@ -338,9 +432,29 @@ __global__ __launch_bounds__(256, 2) void paged_split(PagedAttn a) {
                     o[r][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[r], o[r][j], 0, 0, 0);
                 }
             }
+        };
+
+        // while a step is computed the next one's loads are in flight (where registers hold both), and the page ids
+        // of the one after
+        auto step = [&](Tile& t, Tile& other, int st) {
+            const Pages at_page = here;
+            here = next;
+            if (TWO && st + 1 < mine) load(other, st + 1, here);
+            if (st + 2 < mine) next = pages(st + 2);
+            compute(t, st, at_page);
+            if (!TWO && st + 1 < mine) load(t, st + 1, here);
+        };
+        if constexpr (TWO) {
+            for (int st = at; st < mine; st += 2) {
+                step(ta, tb, st);
+                if (st + 1 < mine) step(tb, ta, st + 1);
+            }
+        } else {
+            for (int st = at; st < mine; ++st) step(ta, ta, st);
         }
 
-        // join the wavefronts: 2 and 3 hand theirs to 0 and 1, then 1 to 0
+        // join the wavefronts: each brings its sums to the rows' maximum and the smallest power of two; 2 and 3 hand
+        // theirs to 0 and 1, and all threads add what those two then hold
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             l[r] = quad_sum(l[r]);
@@ -351,82 +465,73 @@ __global__ __launch_bounds__(256, 2) void paged_split(PagedAttn a) {
         }
         if (lane == 0) wave_up[wave] = vup;
         __syncthreads();
-        int up = wave_up[0];
-#pragma unroll
-        for (int k = 1; k < WAVES; ++k) up = min(up, wave_up[k]);
+        const int up = min(min(wave_up[0], wave_up[1]), min(wave_up[2], wave_up[3]));
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            float mx = wave_m[0][16 * r + n], sum = 0.f;
+            float mx = m[r];
 #pragma unroll
-            for (int k = 1; k < WAVES; ++k) mx = fmaxf(mx, wave_m[k][16 * r + n]);
-            const float base = mx == -INFINITY ? 0.f : mx;
-#pragma unroll
-            for (int k = 0; k < WAVES; ++k) sum += wave_l[k][16 * r + n] * __builtin_amdgcn_exp2f(wave_m[k][16 * r + n] - base);
-            const float f = __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(m[r] - base), up - vup);
+            for (int k = 0; k < WAVES; ++k) mx = fmaxf(mx, wave_m[k][16 * r + n]);
+            const float f = __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(m[r] - (mx == -INFINITY ? 0.f : mx)), up - vup);
 #pragma unroll
             for (int j = 0; j < ND; ++j) o[r][j] *= f;
-            m[r] = mx;
-            l[r] = sum;
         }
+        floatx4* const mine_at = (floatx4*)hand[wave & 1];
+        if (wave >= 2) {
 #pragma unroll
-        for (int half = WAVES / 2; half; half >>= 1) {
-            if (wave >= half && wave < 2 * half) {
-                floatx4* const to = (floatx4*)hand[wave - half];
+            for (int r = 0; r < NR; ++r)
 #pragma unroll
-                for (int r = 0; r < NR; ++r)
-#pragma unroll
-                    for (int j = 0; j < ND; ++j) to[(r * ND + j) * 64 + lane] = o[r][j];
-            }
-            __syncthreads();
-            if (wave < half) {
-                const floatx4* const from = (const floatx4*)hand[wave];
-#pragma unroll
-                for (int r = 0; r < NR; ++r)
-#pragma unroll
-                    for (int j = 0; j < ND; ++j) o[r][j] += from[(r * ND + j) * 64 + lane];
-            }
-            __syncthreads();
+                for (int j = 0; j < ND; ++j) mine_at[(r * ND + j) * 64 + lane] = o[r][j];
         }
+        __syncthreads();
+        if (wave < 2) {
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+#pragma unroll
+                for (int j = 0; j < ND; ++j) mine_at[(r * ND + j) * 64 + lane] += o[r][j];
+        }
+        __syncthreads();
 
-        if (wave == 0) {
-            const long long seg = (before * c.heads) + (long long)h * steps;   // its first step in the line
-            const bool whole = seg >= first && seg + steps <= end;
-            float* const part = a.parts + (2 * w + (seg >= first)) * part_floats<HD, NR>();
+        const long long seg = pl.before * c.heads + (long long)h * steps;   // its first step in the line
+        const bool whole = seg >= first && seg + steps <= end;
+        float* const part = a.parts + (2 * w + (seg >= first)) * part_floats<HD, NR>();
+        {
+            const int col = tid % LPR * 4;
+            // where the row's columns lie: block, lane group, and (one-byte types) every other value of two blocks
+            const int j = ES == 1 ? col / 32 * 2 : col / 16, g4 = ES == 1 ? col % 32 / 8 : col % 16 / 4;
+            const int rows = whole ? a.rows : ROWS;
+            for (int r = tid / LPR; r < rows; r += 256 / LPR) {
+                float mx = wave_m[0][r], sum = 0.f;
 #pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                const int row = 16 * r + n;
-                const int token = (int)lbr_fdiv((unsigned)min(row, a.rows - 1), a.G_m, a.G_s), g = min(row, a.rows - 1) - token * a.G;
-                const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];   // no keys in this range
-                float* const to = whole ? a.out + ((long long)(b * a.H + h * a.G + g) * a.S + token) * c.hd : part + row * HD;
-                if (!whole && kg == 0) {
-                    part[ROWS * HD + row] = m[r];
-                    part[ROWS * HD + ROWS + row] = l[r];
+                for (int k = 1; k < WAVES; ++k) mx = fmaxf(mx, wave_m[k][r]);
+                const float base = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+                for (int k = 0; k < WAVES; ++k) sum += wave_l[k][r] * __builtin_amdgcn_exp2f(wave_m[k][r] - base);
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;   // no keys in this range
+                float v[4];
+                const int p = ((r / 16 * ND + j) * 64 + g4 * 16 + r % 16) * 4;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int q = ES == 1 ? p + (k & 1) * 256 + col % 8 / 2 + (k >> 1) : p + k;
+                    v[k] = __builtin_amdgcn_ldexpf((hand[0][q] + hand[1][q]) * inv, 127 - up);
                 }
-                if (whole && row >= a.rows) continue;
-                const bool vec = !whole || a.vec;
-                const int cols = whole ? c.hd : HD;
-#pragma unroll
-                for (int j = 0; j < ND; j += ES == 1 ? 2 : 1) {
-                    // four (eight) neighbouring columns
-                    constexpr int NC = ES == 1 ? 8 : 4;
-                    const int col = ES == 1 ? (j / 2) * 32 + 8 * kg : j * 16 + 4 * kg;
-                    float v[NC];
-#pragma unroll
-                    for (int k = 0; k < NC; ++k) {
-                        const float e = ES == 1 ? o[r][j + (k & 1)][k >> 1] : o[r][j][k];
-                        v[k] = __builtin_amdgcn_ldexpf(e * inv, 127 - up);
-                        if (whole) v[k] = row_value(a, sp, token, v[k]);
+                if (!whole) {
+                    *(float4*)(part + r * HD + col) = make_float4(v[0], v[1], v[2], v[3]);
+                    if (col == 0) {
+                        part[ROWS * HD + r] = mx;
+                        part[ROWS * HD + ROWS + r] = sum;
                     }
+                    continue;
+                }
+                const int token = (int)lbr_fdiv((unsigned)r, a.G_m, a.G_s), g = r - token * a.G;
+                float* const to = a.out + ((long long)(b * a.H + h * a.G + g) * a.S + token) * hd;
 #pragma unroll
-                    for (int k = 0; k < NC; k += 4) {
-                        if (vec && col + k + 4 <= cols) {
-                            *(float4*)(to + col + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
-                        } else {
+                for (int k = 0; k < 4; ++k) v[k] = row_value(a, sp, token, v[k]);
+                if (a.vec && col < hd) {
+                    *(float4*)(to + col) = make_float4(v[0], v[1], v[2], v[3]);
+                } else {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (col + k + e < cols) to[col + k + e] = v[k + e];
-                        }
-                    }
+                    for (int k = 0; k < 4; ++k)
+                        if (col + k < hd) to[col + k] = v[k];
                 }
             }
         }
@@ -435,43 +540,63 @@ __global__ __launch_bounds__(256, 2) void paged_split(PagedAttn a) {
         at = 0;
         if (++h == c.heads && x < end) {
             h = 0;
-            before += steps;
-            steps = steps_of(a, ++b);
+            const int lane1 = b + 1 - line.first;
+            if (lane1 == 64) line_next(a, line);
+            pl = line_place(line, lane1 & 63);
         }
     }
 }
 
-// Joins the partial results of a segment that ranges cut: one workgroup a (sequence, K/V head, 16 rows).
+// Joins the partial results of a segment that ranges cut, gridDim.y workgroups its rows: HD / 4 threads across a
+// row, and the results dealt out over the rest, which add up in LDS.
 template <int HD, int NR>
 __global__ __launch_bounds__(256) void paged_merge(PagedAttn a, long long ranges) {
-    constexpr int ROWS = 16 * NR;
-    __shared__ Line line;
+    constexpr int ROWS = 16 * NR, LANES = HD / 4, SLICES = 256 / LANES;
+    __shared__ float slice_m[SLICES], slice_l[SLICES];
+    __shared__ floatx4 slice_o[SLICES][LANES];
     const int tid = threadIdx.x;
     const PagedCache& c = a.c;
     const int b = blockIdx.x / c.heads, h = blockIdx.x % c.heads;
-    line_build(a, line);
-    // steps before sequence b: those before its block of sequences, and of the block's before it
-    const int per = (a.B + 255) / 256;
-    long long before = line.before[b / per];
-    for (int k = b / per * per; k < b; ++k) before += steps_of(a, k);
-    const int steps = steps_of(a, b);
-    const long long T = line.before[256] * c.heads, W = min(ranges, T), seg = before * c.heads + (long long)h * steps;
-    const long long w0 = range_of(seg, W, T), w1 = range_of(seg + steps - 1, W, T);
+    Line line;
+    const long long T = line_begin(a, line) * c.heads, W = min(ranges, T);
+    while (b >= line.first + 64) line_next(a, line);
+    const Place pl = line_place(line, b - line.first);
+    const long long seg = pl.before * c.heads + (long long)h * pl.steps;
+    const int w0 = (int)range_of(seg, W, T), w1 = (int)range_of(seg + pl.steps - 1, W, T);
     if (w0 == w1) return;   // finished by its range
-    const Span sp = span_of(a, b);
-    constexpr int LANES = HD / 4;    // threads a row
-    for (int row = blockIdx.y * 16 + tid / LANES; row < min(a.rows, (int)blockIdx.y * 16 + 16); row += 256 / LANES) {
-        const int col = tid % LANES * 4;
+    const int lane = tid % LANES, slice = tid / LANES;
+    for (int row = blockIdx.y; row < a.rows; row += gridDim.y) {
         float m = -INFINITY, l = 0.f;
         floatx4 o = {0.f, 0.f, 0.f, 0.f};
-        for (long long w = w0; w <= w1; ++w) {
-            const float* const part = a.parts + (2 * w + (w == w0)) * part_floats<HD, NR>();
-            const float pm = part[ROWS * HD + row], pl = part[ROWS * HD + ROWS + row];
-            const floatx4 v = *(const floatx4*)(part + row * HD + col);
-            const float mx = fmaxf(m, pm), base = mx == -INFINITY ? 0.f : mx;
-            const float f = __builtin_amdgcn_exp2f(m - base), g = __builtin_amdgcn_exp2f(pm - base) * pl;
-            o = o * f + v * g;
-            l = l * f + g;
+        constexpr int AHEAD = 4;   // loads in flight
+        for (int w = w0 + slice; w <= w1; w += AHEAD * SLICES) {
+            float pm[AHEAD], ps[AHEAD];
+            floatx4 v[AHEAD];
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                const int at = min(w + k * SLICES, w1);
+                const float* const part = a.parts + (2LL * at + (at == w0)) * part_floats<HD, NR>();
+                pm[k] = part[ROWS * HD + row];
+                ps[k] = w + k * SLICES <= w1 ? part[ROWS * HD + ROWS + row] : 0.f;
+                v[k] = *(const floatx4*)(part + row * HD + 4 * lane);
+            }
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k)
+                if (w + k * SLICES <= w1) merge_part(m, l, o, pm[k], ps[k], v[k]);
+        }
+        __syncthreads();   // of the row before
+        if (lane == 0) {
+            slice_m[slice] = m;
+            slice_l[slice] = l;
+        }
+        slice_o[slice][lane] = o;
+        __syncthreads();
+        if (slice) continue;
+        for (int k = 1; k < SLICES; ++k) {   // sums, not weighted means
+            const float mx = fmaxf(m, slice_m[k]), base = mx == -INFINITY ? 0.f : mx;
+            const float f = __builtin_amdgcn_exp2f(m - base), g = __builtin_amdgcn_exp2f(slice_m[k] - base);
+            o = o * f + slice_o[k][lane] * g;
+            l = l * f + slice_l[k] * g;
             m = mx;
         }
         const float inv = 1.f / l;
@@ -479,17 +604,18 @@ __global__ __launch_bounds__(256) void paged_merge(PagedAttn a, long long ranges
         float* const to = a.out + ((long long)(b * a.H + h * a.G + g) * a.S + token) * c.hd;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (col + e < c.hd) to[col + e] = row_value(a, sp, token, o[e] * inv);
+            if (4 * lane + e < c.hd) to[4 * lane + e] = row_value(a, pl.sp, token, o[e] * inv);
     }
 }
 
 // ---------------------------------------------------------------- launch
 
-// Ranges of the split kernel: two workgroups a CU, as many as there can be steps.
+// Ranges of the split kernel: the workgroups that the chip holds at once (Step::i[11] a CU), or as many as there can
+// be steps.
 long long split_ranges(const Step& s) {
-    const int cus = lbr_device_cus() > 0 ? lbr_device_cus() : 256;
+    const long long wgs = s.i[11] * (lbr_device_cus() > 0 ? lbr_device_cus() : 256);
     const long long steps = (((s.i[6] << s.i[4]) + STEP_WG - 1) / STEP_WG) * s.i[1] * s.i[2];
-    return steps < 2LL * cus ? steps : 2LL * cus;
+    return steps < wgs ? steps : wgs;
 }
 // Whether a segment can be longer than a step, and so cut.
 bool split_cuts(const Step& s) { return (s.i[6] << s.i[4]) > STEP_WG; }
@@ -500,18 +626,27 @@ void launch_split(const Step& s, hipStream_t st) {
     const long long W = split_ranges(s);
     if (W <= 0 || a.rows <= 0) return;
     hipLaunchKernelGGL((paged_split<TYPE, HD, NR>), dim3((unsigned)W), dim3(256), 0, st, a);
-    if (split_cuts(s))
-        hipLaunchKernelGGL((paged_merge<HD, NR>), dim3((unsigned)(a.B * a.c.heads), (unsigned)((a.rows + 15) / 16)),
-                           dim3(256), 0, st, a, W);
+    if (split_cuts(s)) {
+        // about two workgroups a CU: most find that their segment was not cut, which takes them as long as a row does
+        const long long segments = (long long)a.B * a.c.heads, each = 512 / segments;
+        const unsigned rows = (unsigned)(each < 1 ? 1 : each < a.rows ? each : a.rows);
+        hipLaunchKernelGGL((paged_merge<HD, NR>), dim3((unsigned)segments, rows), dim3(256), 0, st, a, W);
+    }
 }
 
+template <int TYPE, int HD, int NR>
+void choose(Step* s) {
+    s->i[11] = split_occupancy<TYPE, HD, NR>();
+    s->ws_bytes = split_cuts(*s) ? (size_t)(split_ranges(*s) * 2 * part_floats<HD, NR>()) * sizeof(float) : 0;
+    s->run = launch_split<TYPE, HD, NR>;
+}
 template <int TYPE, int HD>
-step_fn split_rows(int nr) {
-    return nr == 1 ? launch_split<TYPE, HD, 1> : nr == 2 ? launch_split<TYPE, HD, 2> : launch_split<TYPE, HD, 4>;
+void choose_rows(Step* s, int nr) {
+    nr == 1 ? choose<TYPE, HD, 1>(s) : choose<TYPE, HD, 2>(s);
 }
 template <int TYPE>
-step_fn split_for(int hd, int nr) {
-    return hd <= 64 ? split_rows<TYPE, 64>(nr) : hd <= 128 ? split_rows<TYPE, 128>(nr) : split_rows<TYPE, 256>(nr);
+void choose_split(Step* s, int hd, int nr) {
+    hd <= 64 ? choose_rows<TYPE, 64>(s, nr) : hd <= 128 ? choose_rows<TYPE, 128>(s, nr) : choose_rows<TYPE, 256>(s, nr);
 }
 
 }  // namespace
@@ -546,14 +681,15 @@ int decode_paged_attention(const OpNode* n, Step* s) {
     const int hd = (int)s->i[3];
     const long long rows = s->i[8] / s->i[2] * s->i[7];
     s->i[9] = hd % 4 == 0 && lbr_aligned(s->in[4], 16) && lbr_aligned(s->out, 16);
-    if (rows <= 64) {
-        const int nr = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-        const int wide = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
-        s->ws_bytes = split_cuts(*s) ? (size_t)(split_ranges(*s) * 2 * 16 * nr * (wide + 2)) * sizeof(float) : 0;
-        s->run = s->i[0] == LBR_CACHE_F32   ? split_for<LBR_CACHE_F32>(hd, nr)
-                 : s->i[0] == LBR_CACHE_F16 ? split_for<LBR_CACHE_F16>(hd, nr)
-                 : s->i[0] == LBR_CACHE_I8  ? split_for<LBR_CACHE_I8>(hd, nr)
-                                            : split_for<LBR_CACHE_E4M3>(hd, nr);
+    // At most 32 rows a K/V head are split over the keys, in one or two blocks of 16; more go in tiles.  16 sequences
+    // of 2048 keys, 32/8 heads of 128, 20 rows: 41 µs split and 52 in tiles (int8), 43 and 48 (float16), 76 and 78
+    // (float32); 40 rows (in four blocks): 68 and 56, 99 and 52, 134 and 86.
+    if (rows <= 32) {
+        const int nr = rows <= 16 ? 1 : 2;
+        if (s->i[0] == LBR_CACHE_F32) choose_split<LBR_CACHE_F32>(s, hd, nr);
+        else if (s->i[0] == LBR_CACHE_F16) choose_split<LBR_CACHE_F16>(s, hd, nr);
+        else if (s->i[0] == LBR_CACHE_I8) choose_split<LBR_CACHE_I8>(s, hd, nr);
+        else choose_split<LBR_CACHE_E4M3>(s, hd, nr);
         s->name = "paged_split";
         return LBR_OK;
     }

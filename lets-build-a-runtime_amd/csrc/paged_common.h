@@ -44,6 +44,25 @@ __device__ __forceinline__ char* cache_head(const PagedCache& c, int b, int h, l
     return c.base + page * c.page_bytes + (long long)h * c.head_bytes;
 }
 
+// Max over the aligned groups of G lanes that hold a row.
+template <int G>
+__device__ __forceinline__ unsigned row_max_bits(unsigned v) {
+    static_assert(G == 16 || G == 32 || G == 64, "lanes of a row");
+    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false));
+    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, false));
+    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, false));
+    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, false));
+    if (G >= 32) {
+        auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = max((unsigned)a[0], (unsigned)a[1]);
+    }
+    if (G == 64) {
+        auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = max((unsigned)a[0], (unsigned)a[1]);
+    }
+    return v;
+}
+
 // Fields of Step for the cache ops: in[0] = cache, in[1] = table, in[2] = start, in[3] = count, in[4]
 // = K or Q, in[5] = V; i[0] = type, i[1] = B, i[2] = heads, i[3] = head_dim, i[4] = log2 page_size,
 // i[5] = pages, i[6] = pages of a table row, i[7] = S or T, i[8] = query heads, i[9] = 16-byte rows;

@@ -1,4 +1,4 @@
-// paged_tiles.hip — attention over the paged cache: chunks of more than 64 rows a K/V head.
+// paged_tiles.hip — attention over the paged cache: chunks of more than 32 rows a K/V head.
 #include "paged_attention.h"
 
 #include <type_traits>
@@ -404,7 +404,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void paged_tiles(PagedAttn a
         part[ROWS_WG * HD + wave * 32 + n] = m;
         part[ROWS_WG * HD + ROWS_WG + wave * 32 + n] = __builtin_amdgcn_ldexpf(l, 127 - vup);
     }
-    if (whole && row >= a.rows) return;
+    if (row >= a.rows) return;
     float* const to = whole ? a.out + qat : part + (wave * 32 + n) * HD;
     const int cols = whole ? c.hd : HD;
     const bool vec = !whole || a.vec;
@@ -438,15 +438,20 @@ __global__ __launch_bounds__(256) void paged_tiles_merge(PagedAttn a, int tiles,
     if (row >= a.rows) return;
     float m = -INFINITY, l = 0.f;
     floatx4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < splits; ++k) {
-        const float* const part = a.parts + ((long long)k * gridDim.x + blockIdx.x) * tile_floats<HD>();
-        const float pm = part[ROWS_WG * HD + r], pl = part[ROWS_WG * HD + ROWS_WG + r];
-        const floatx4 v = *(const floatx4*)(part + r * HD + col);
-        const float mx = fmaxf(m, pm), base = mx == -INFINITY ? 0.f : mx;
-        const float f = __builtin_amdgcn_exp2f(m - base), g = __builtin_amdgcn_exp2f(pm - base) * pl;
-        o = o * f + v * g;
-        l = l * f + g;
-        m = mx;
+    constexpr int AHEAD = 8;   // loads in flight
+    for (int k0 = 0; k0 < splits; k0 += AHEAD) {
+        float pm[AHEAD], ps[AHEAD];
+        floatx4 v[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const float* const part = a.parts + ((long long)min(k0 + k, splits - 1) * gridDim.x + blockIdx.x) * tile_floats<HD>();
+            pm[k] = part[ROWS_WG * HD + r];
+            ps[k] = part[ROWS_WG * HD + ROWS_WG + r];
+            v[k] = *(const floatx4*)(part + r * HD + col);
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+            if (k0 + k < splits) merge_part(m, l, o, pm[k], ps[k], v[k]);
     }
     const float inv = 1.f / l;
     const Span sp = span_of(a, b);
