@@ -28,7 +28,7 @@ __device__ __forceinline__ int steps_of(const Span& s) { return max(1, (s.keys +
 struct Line {
     Span sp;
     int first, steps, run;
-    long long before;   // steps of the sequences before `first`
+    int before;   // steps of the sequences before `first`
 };
 
 __device__ __forceinline__ void line_load(const PagedAttn& a, Line& ln) {
@@ -42,8 +42,8 @@ __device__ __forceinline__ void line_load(const PagedAttn& a, Line& ln) {
     }
 }
 // From the first sequence on, and all steps of a head.
-__device__ __forceinline__ long long line_begin(const PagedAttn& a, Line& ln) {
-    long long all = 0;
+__device__ __forceinline__ int line_begin(const PagedAttn& a, Line& ln) {
+    int all = 0;
     for (int first = (a.B - 1) / 64 * 64; first >= 0; first -= 64) {
         ln.first = first;
         line_load(a, ln);
@@ -62,7 +62,7 @@ __device__ __forceinline__ void line_next(const PagedAttn& a, Line& ln) {
 struct Place {
     int b, steps;
     Span sp;
-    long long before;
+    int before;
 };
 __device__ __forceinline__ Place line_place(const Line& ln, int lane) {
     Place p;
@@ -75,15 +75,15 @@ __device__ __forceinline__ Place line_place(const Line& ln, int lane) {
     return p;
 }
 // The sequence that step x of all heads' falls to; x lies in the line.
-__device__ __forceinline__ Place line_seek(const PagedAttn& a, Line& ln, long long x) {
-    const long long heads = a.c.heads;
+__device__ __forceinline__ Place line_seek(const PagedAttn& a, Line& ln, int x) {
+    const int heads = a.c.heads;
     while (x >= (ln.before + __builtin_amdgcn_readlane(ln.run, 63)) * heads) line_next(a, ln);
     return line_place(ln, __builtin_ctzll(__ballot(x < (ln.before + ln.run) * heads)));
 }
 
 // Range w of W ≤ T over T steps starts at w·T/W; the range that step x falls to.
-__device__ __forceinline__ long long range_start(long long w, long long W, long long T) { return w * T / W; }
-__device__ __forceinline__ long long range_of(long long x, long long W, long long T) { return ((x + 1) * W - 1) / T; }
+__device__ __forceinline__ int range_start(int w, int W, int T) { return (int)((unsigned long long)w * T / W); }
+__device__ __forceinline__ int range_of(int x, int W, int T) { return (int)(((unsigned long long)x * W + W - 1) / T); }
 
 // Floats of a partial result: rows of outputs, then each row's maximum and sum.
 template <int HD, int NR>
@@ -94,14 +94,15 @@ constexpr int part_floats() { return 16 * NR * (HD + 2); }
 // workgroups of one tile 63 µs, one of two 80.)
 template <int TYPE, int HD, int NR>
 constexpr int split_registers(int tiles) {
-    return tiles * (HD * cache_elem(TYPE) / 4 + 16) + NR * HD / 4 + 64 + 16 * NR;
+    return tiles * (HD * cache_elem(TYPE) / 4 + 16) + NR * HD / 4 + 64 + 20 * NR;
 }
 template <int TYPE, int HD, int NR>
 constexpr int split_occupancy() { return split_registers<TYPE, HD, NR>(1) <= 256 ? 2 : 1; }
 template <int TYPE, int HD, int NR>
-constexpr int split_tiles() { return split_registers<TYPE, HD, NR>(2) <= (split_occupancy<TYPE, HD, NR>() == 2 ? 256 : 480) ? 2 : 1; }
+constexpr int split_tiles() { return split_registers<TYPE, HD, NR>(2) <= (split_occupancy<TYPE, HD, NR>() == 2 ? 256 : 440) ? 2 : 1; }
 
-template <int TYPE, int HD, int NR>
+// EXACT: rows have HD columns; else loads of columns that they do not have take the first ones (q is zero there).
+template <int TYPE, int HD, int NR, bool EXACT>
 __global__ __launch_bounds__(256, (split_occupancy<TYPE, HD, NR>())) void paged_split(PagedAttn a) {
     constexpr int ES = cache_elem(TYPE);
     constexpr int NK = HD / 32;          // MFMA steps over the columns
@@ -110,11 +111,15 @@ __global__ __launch_bounds__(256, (split_occupancy<TYPE, HD, NR>())) void paged_
     constexpr int ROWS = 16 * NR;
     constexpr bool TWO = split_tiles<TYPE, HD, NR>() == 2;
     constexpr int LPR = HD / 4;          // threads of a row where all load or store it
-    __shared__ __attribute__((aligned(16))) _Float16 q_lds[2 * NR * NK * 512];   // [16 rows][MFMA step][h, l][lane][8]
-    __shared__ float q_scale[ROWS];
+    constexpr int PAD = HD + 4;          // floats of a row in `hand`: 16 rows' float4s then hit every bank once
+    // q until the last step, [16 rows][MFMA step][h, l][lane][8]; then each wavefront's sums, `hand`[wave][row][PAD]
+    __shared__ __attribute__((aligned(16))) char shared[WAVES * ROWS * PAD * 4];
+    static_assert(2 * NR * NK * 1024 <= sizeof(shared), "q fits where the sums go");
+    _Float16* const q_lds = (_Float16*)shared;
+    float* const hand = (float*)shared;
+    __shared__ float q_scale[ROWS], row_m[ROWS], row_l[ROWS];
     __shared__ float wave_m[WAVES][ROWS], wave_l[WAVES][ROWS];
     __shared__ int wave_up[WAVES];
-    __shared__ __attribute__((aligned(16))) float hand[2][ROWS * HD];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, kg = lane >> 4;
@@ -122,26 +127,24 @@ __global__ __launch_bounds__(256, (split_occupancy<TYPE, HD, NR>())) void paged_
     const int page = 1 << c.shift, mask = page - 1;
 
     Line line;
-    const long long T = line_begin(a, line) * c.heads, W = min((long long)gridDim.x, T), w = blockIdx.x;
+    const int T = line_begin(a, line) * c.heads, W = min((int)gridDim.x, T), w = blockIdx.x;
     if (w >= W) return;
-    long long x = range_start(w, W, T);
-    const long long first = x, end = range_start(w + 1, W, T);
+    int x = range_start(w, W, T);
+    const int first = x, end = range_start(w + 1, W, T);
     Place pl = line_seek(a, line, x);
-    int h = (int)((x - pl.before * c.heads) / pl.steps);
-    int at = (int)(x - pl.before * c.heads - (long long)h * pl.steps);
+    int h = (x - pl.before * c.heads) / pl.steps;
+    int at = x - pl.before * c.heads - h * pl.steps;
 
-    // columns of a lane's loads, clamped to the row (q is zero behind it)
-    int koff[NK], voff[ND];
-#pragma unroll
-    for (int j = 0; j < NK; ++j) {
+    const int hdp = EXACT ? HD : c.hdp;
+    // bytes into a K row and into a V group of a lane's loads
+    auto koff = [&](int j) {
         const int col = ES == 1 ? (j / 2) * 64 + kg * 16 + (j % 2) * 8 : j * 32 + kg * 8;
-        koff[j] = (col < c.hdp ? col : 0) * ES;
-    }
-#pragma unroll
-    for (int j = 0; j < ND; ++j) {
+        return (EXACT || col < hdp ? col : 0) * ES;
+    };
+    auto voff = [&](int j) {
         const int col = ES == 1 ? (j / 2) * 32 + 2 * n + (j & 1) : j * 16 + n;
-        voff[j] = (col < c.hdp ? col : 0) * 8 * ES;
-    }
+        return (EXACT || col < hdp ? col : 0) * 8 * ES;
+    };
 
     // a wavefront's 32 keys of a step, as loaded
     struct Tile {
@@ -155,7 +158,7 @@ __global__ __launch_bounds__(256, (split_occupancy<TYPE, HD, NR>())) void paged_
     while (x < end) {   // segments
         const Span sp = pl.sp;
         const int b = pl.b, steps = pl.steps;
-        const int stop = (int)min((long long)steps, at + (end - x));   // steps at .. stop − 1 of this segment
+        const int stop = min(steps, at + (end - x));   // steps at .. stop − 1 of this segment
         // the wavefront's own: those that begin before the end
         const int mine = min(stop, (sp.keys - wave * STEP + STEP_WG - 1) / STEP_WG);
         const int lastg = (sp.keys - 1) & ~7;
@@ -178,14 +181,14 @@ __global__ __launch_bounds__(256, (split_occupancy<TYPE, HD, NR>())) void paged_
             const char* const hv = kg >= 2 ? hi : lo;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const char* const row = hk + ((gk & mask) + 4 * u + (n & 3)) * c.hdp * ES;
+                const char* const row = hk + ((gk & mask) + 4 * u + (n & 3)) * hdp * ES;
 #pragma unroll
                 for (int j = 0; j < NK; ++j) {
                     if (ES == 1) {
-                        if (j % 2 == 0) t.k[u][j / 2] = *(const uint4*)(row + koff[j]);
+                        if (j % 2 == 0) t.k[u][j / 2] = *(const uint4*)(row + koff(j));
                     } else {
 #pragma unroll
-                        for (int e = 0; e < ES / 2; ++e) t.k[u][j * (ES / 2) + e] = *(const uint4*)(row + koff[j] + 16 * e);
+                        for (int e = 0; e < ES / 2; ++e) t.k[u][j * (ES / 2) + e] = *(const uint4*)(row + koff(j) + 16 * e);
                     }
                 }
             }
@@ -196,35 +199,26 @@ __global__ __launch_bounds__(256, (split_occupancy<TYPE, HD, NR>())) void paged_
                 t.ks[4 * e] = u.x; t.ks[4 * e + 1] = u.y; t.ks[4 * e + 2] = u.z; t.ks[4 * e + 3] = u.w;
                 t.vs[4 * e] = v.x; t.vs[4 * e + 1] = v.y; t.vs[4 * e + 2] = v.z; t.vs[4 * e + 3] = v.w;
             }
-            const char* const vb = hv + c.part + (gv & mask) * c.hdp * ES;
+            const char* const vb = hv + c.part + (gv & mask) * hdp * ES;
 #pragma unroll
             for (int j = 0; j < ND; ++j) {
                 if (ES == 1) {
-                    if (j % 2 == 0) t.v[j / 2] = *(const uint4*)(vb + voff[j]);
+                    if (j % 2 == 0) t.v[j / 2] = *(const uint4*)(vb + voff(j));
                 } else {
 #pragma unroll
-                    for (int e = 0; e < ES / 2; ++e) t.v[j * (ES / 2) + e] = *(const uint4*)(vb + voff[j] + 16 * e);
+                    for (int e = 0; e < ES / 2; ++e) t.v[j * (ES / 2) + e] = *(const uint4*)(vb + voff(j) + 16 * e);
                 }
             }
         };
-        Tile ta, tb;
-        Pages here = {0, 0}, next = {0, 0};   // of the step being computed, and of the next
-        if (at < mine) {
-            here = pages(at);
-            if (at + 1 < mine) next = pages(at + 1);
-            load(ta, at, here);
-        }
-
         // rows of q into LDS: two halves, scaled, in the order of the MFMAs' operands
         int hd = c.hd;
         asm volatile("" : "+s"(hd));   // or what depends on it alone is worked out ahead of the loop, and spilled
+        const int col = tid % LPR * 4;
+        constexpr int EACH = ROWS * LPR / 256;   // rows a thread
+        float v[EACH][4];
         {
-            const int col = tid % LPR * 4;
-            const int j = ES == 1 ? col / 64 * 2 + col % 16 / 8 : col / 32, g4 = ES == 1 ? col % 64 / 16 : col % 32 / 8;
-            constexpr int EACH = ROWS * LPR / 256;   // rows a thread
-            float v[EACH][4];
 #pragma unroll
-            for (int i = 0; i < EACH; ++i) {   // all loads go out together
+            for (int i = 0; i < EACH; ++i) {   // all loads go out together, ahead of the first tile's
                 const int r = i * (256 / LPR) + tid / LPR;
                 const int token = (int)lbr_fdiv((unsigned)min(r, a.rows - 1), a.G_m, a.G_s), g = min(r, a.rows - 1) - token * a.G;
                 const float* const qr = a.q + ((long long)(b * a.H + h * a.G + g) * a.S + token) * hd;
@@ -244,6 +238,17 @@ __global__ __launch_bounds__(256, (split_occupancy<TYPE, HD, NR>())) void paged_
                     }
                 }
             }
+        }
+        Tile ta, tb;
+        Pages here = {0, 0}, next = {0, 0};   // of the step being computed, and of the next
+        if (at < mine) {
+            here = pages(at);
+            if (at + 1 < mine) next = pages(at + 1);
+            load(ta, at, here);
+        }
+
+        {
+            const int j = ES == 1 ? col / 64 * 2 + col % 16 / 8 : col / 32, g4 = ES == 1 ? col % 64 / 16 : col % 32 / 8;
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
                 const int r = i * (256 / LPR) + tid / LPR;
@@ -453,8 +458,8 @@ __global__ __launch_bounds__(256, (split_occupancy<TYPE, HD, NR>())) void paged_
             for (int st = at; st < mine; ++st) step(ta, ta, st);
         }
 
-        // join the wavefronts: each brings its sums to the rows' maximum and the smallest power of two; 2 and 3 hand
-        // theirs to 0 and 1, and all threads add what those two then hold
+        // join the wavefronts: each brings its sums to the rows' maximum and the smallest power of two and hands them
+        // over, and all threads add up
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             l[r] = quad_sum(l[r]);
@@ -472,69 +477,65 @@ __global__ __launch_bounds__(256, (split_occupancy<TYPE, HD, NR>())) void paged_
 #pragma unroll
             for (int k = 0; k < WAVES; ++k) mx = fmaxf(mx, wave_m[k][16 * r + n]);
             const float f = __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(m[r] - (mx == -INFINITY ? 0.f : mx)), up - vup);
+            float* const to = hand + ((wave * ROWS) + 16 * r + n) * PAD;
+            // a lane's accumulators are columns 4·kg .. of a block, or every other one of 8·kg .. of two
 #pragma unroll
-            for (int j = 0; j < ND; ++j) o[r][j] *= f;
-        }
-        floatx4* const mine_at = (floatx4*)hand[wave & 1];
-        if (wave >= 2) {
-#pragma unroll
-            for (int r = 0; r < NR; ++r)
-#pragma unroll
-                for (int j = 0; j < ND; ++j) mine_at[(r * ND + j) * 64 + lane] = o[r][j];
-        }
-        __syncthreads();
-        if (wave < 2) {
-#pragma unroll
-            for (int r = 0; r < NR; ++r)
-#pragma unroll
-                for (int j = 0; j < ND; ++j) mine_at[(r * ND + j) * 64 + lane] += o[r][j];
-        }
-        __syncthreads();
-
-        const long long seg = pl.before * c.heads + (long long)h * steps;   // its first step in the line
-        const bool whole = seg >= first && seg + steps <= end;
-        float* const part = a.parts + (2 * w + (seg >= first)) * part_floats<HD, NR>();
-        {
-            const int col = tid % LPR * 4;
-            // where the row's columns lie: block, lane group, and (one-byte types) every other value of two blocks
-            const int j = ES == 1 ? col / 32 * 2 : col / 16, g4 = ES == 1 ? col % 32 / 8 : col % 16 / 4;
-            const int rows = whole ? a.rows : ROWS;
-            for (int r = tid / LPR; r < rows; r += 256 / LPR) {
-                float mx = wave_m[0][r], sum = 0.f;
-#pragma unroll
-                for (int k = 1; k < WAVES; ++k) mx = fmaxf(mx, wave_m[k][r]);
-                const float base = mx == -INFINITY ? 0.f : mx;
-#pragma unroll
-                for (int k = 0; k < WAVES; ++k) sum += wave_l[k][r] * __builtin_amdgcn_exp2f(wave_m[k][r] - base);
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;   // no keys in this range
-                float v[4];
-                const int p = ((r / 16 * ND + j) * 64 + g4 * 16 + r % 16) * 4;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int q = ES == 1 ? p + (k & 1) * 256 + col % 8 / 2 + (k >> 1) : p + k;
-                    v[k] = __builtin_amdgcn_ldexpf((hand[0][q] + hand[1][q]) * inv, 127 - up);
-                }
-                if (!whole) {
-                    *(float4*)(part + r * HD + col) = make_float4(v[0], v[1], v[2], v[3]);
-                    if (col == 0) {
-                        part[ROWS * HD + r] = mx;
-                        part[ROWS * HD + ROWS + r] = sum;
-                    }
-                    continue;
-                }
-                const int token = (int)lbr_fdiv((unsigned)r, a.G_m, a.G_s), g = r - token * a.G;
-                float* const to = a.out + ((long long)(b * a.H + h * a.G + g) * a.S + token) * hd;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = row_value(a, sp, token, v[k]);
-                if (a.vec && col < hd) {
-                    *(float4*)(to + col) = make_float4(v[0], v[1], v[2], v[3]);
+            for (int j = 0; j < ND; j += ES == 1 ? 2 : 1) {
+                const floatx4 x = o[r][j] * f;
+                if constexpr (ES == 1) {
+                    const floatx4 y = o[r][j + 1] * f;
+                    *(floatx4*)(to + j * 16 + 8 * kg) = floatx4{x[0], y[0], x[1], y[1]};
+                    *(floatx4*)(to + j * 16 + 8 * kg + 4) = floatx4{x[2], y[2], x[3], y[3]};
                 } else {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (col + k < hd) to[col + k] = v[k];
+                    *(floatx4*)(to + j * 16 + 4 * kg) = x;
                 }
             }
         }
+        if (tid < ROWS) {
+            float mx = wave_m[0][tid], sum = 0.f;
+#pragma unroll
+            for (int k = 1; k < WAVES; ++k) mx = fmaxf(mx, wave_m[k][tid]);
+            const float base = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+            for (int k = 0; k < WAVES; ++k) sum += wave_l[k][tid] * __builtin_amdgcn_exp2f(wave_m[k][tid] - base);
+            row_m[tid] = mx;
+            row_l[tid] = sum;
+        }
+        __syncthreads();
+
+        const int seg = pl.before * c.heads + h * steps;   // its first step in the line
+        const bool whole = seg >= first && seg + steps <= end;
+        float* const part = a.parts + (2LL * w + (seg >= first)) * part_floats<HD, NR>();
+        for (int r = tid / LPR; r < a.rows; r += 256 / LPR) {
+            const float sum = row_l[r];
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;   // no keys in this range
+            floatx4 t = *(const floatx4*)(hand + r * PAD + col);
+#pragma unroll
+            for (int k = 1; k < WAVES; ++k) t += *(const floatx4*)(hand + (k * ROWS + r) * PAD + col);
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = __builtin_amdgcn_ldexpf(t[k] * inv, 127 - up);
+            if (!whole) {
+                *(float4*)(part + r * HD + col) = make_float4(v[0], v[1], v[2], v[3]);
+                if (col == 0) {
+                    part[ROWS * HD + r] = row_m[r];
+                    part[ROWS * HD + ROWS + r] = sum;
+                }
+                continue;
+            }
+            const int token = (int)lbr_fdiv((unsigned)r, a.G_m, a.G_s), g = r - token * a.G;
+            float* const to = a.out + ((long long)(b * a.H + h * a.G + g) * a.S + token) * hd;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = row_value(a, sp, token, v[k]);
+            if (a.vec && col < hd) {
+                *(float4*)(to + col) = make_float4(v[0], v[1], v[2], v[3]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (col + k < hd) to[col + k] = v[k];
+            }
+        }
+        if (stop - at + x < end) __syncthreads();   // the next segment's q goes where the sums are
         // the next segment
         x += stop - at;
         at = 0;
@@ -550,7 +551,7 @@ __global__ __launch_bounds__(256, (split_occupancy<TYPE, HD, NR>())) void paged_
 // Joins the partial results of a segment that ranges cut, gridDim.y workgroups its rows: HD / 4 threads across a
 // row, and the results dealt out over the rest, which add up in LDS.
 template <int HD, int NR>
-__global__ __launch_bounds__(256) void paged_merge(PagedAttn a, long long ranges) {
+__global__ __launch_bounds__(256) void paged_merge(PagedAttn a, int ranges) {
     constexpr int ROWS = 16 * NR, LANES = HD / 4, SLICES = 256 / LANES;
     __shared__ float slice_m[SLICES], slice_l[SLICES];
     __shared__ floatx4 slice_o[SLICES][LANES];
@@ -558,11 +559,11 @@ __global__ __launch_bounds__(256) void paged_merge(PagedAttn a, long long ranges
     const PagedCache& c = a.c;
     const int b = blockIdx.x / c.heads, h = blockIdx.x % c.heads;
     Line line;
-    const long long T = line_begin(a, line) * c.heads, W = min(ranges, T);
+    const int T = line_begin(a, line) * c.heads, W = min(ranges, T);
     while (b >= line.first + 64) line_next(a, line);
     const Place pl = line_place(line, b - line.first);
-    const long long seg = pl.before * c.heads + (long long)h * pl.steps;
-    const int w0 = (int)range_of(seg, W, T), w1 = (int)range_of(seg + pl.steps - 1, W, T);
+    const int seg = pl.before * c.heads + h * pl.steps;
+    const int w0 = range_of(seg, W, T), w1 = range_of(seg + pl.steps - 1, W, T);
     if (w0 == w1) return;   // finished by its range
     const int lane = tid % LANES, slice = tid / LANES;
     for (int row = blockIdx.y; row < a.rows; row += gridDim.y) {
@@ -625,12 +626,14 @@ void launch_split(const Step& s, hipStream_t st) {
     const PagedAttn a = attn_args(s);
     const long long W = split_ranges(s);
     if (W <= 0 || a.rows <= 0) return;
-    hipLaunchKernelGGL((paged_split<TYPE, HD, NR>), dim3((unsigned)W), dim3(256), 0, st, a);
+    if (a.c.hdp == HD) hipLaunchKernelGGL((paged_split<TYPE, HD, NR, true>), dim3((unsigned)W), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((paged_split<TYPE, HD, NR, false>), dim3((unsigned)W), dim3(256), 0, st, a);
     if (split_cuts(s)) {
-        // about two workgroups a CU: most find that their segment was not cut, which takes them as long as a row does
-        const long long segments = (long long)a.B * a.c.heads, each = 512 / segments;
+        // at most the workgroups that the chip holds at once: a row takes one about as long as finding out that a
+        // segment was not cut
+        const long long segments = (long long)a.B * a.c.heads, each = 2048 / segments;
         const unsigned rows = (unsigned)(each < 1 ? 1 : each < a.rows ? each : a.rows);
-        hipLaunchKernelGGL((paged_merge<HD, NR>), dim3((unsigned)segments, rows), dim3(256), 0, st, a, W);
+        hipLaunchKernelGGL((paged_merge<HD, NR>), dim3((unsigned)segments, rows), dim3(256), 0, st, a, (int)W);
     }
 }
 
@@ -646,7 +649,7 @@ void choose_rows(Step* s, int nr) {
 }
 template <int TYPE>
 void choose_split(Step* s, int hd, int nr) {
-    hd <= 64 ? choose_rows<TYPE, 64>(s, nr) : hd <= 128 ? choose_rows<TYPE, 128>(s, nr) : choose_rows<TYPE, 256>(s, nr);
+    hd <= 64 ? choose_rows<TYPE, 64>(s, nr) : hd <= 128 ? choose_rows<TYPE, 128>(s, nr) : choose<TYPE, 256, 1>(s);
 }
 
 }  // namespace
@@ -684,7 +687,12 @@ int decode_paged_attention(const OpNode* n, Step* s) {
     // At most 32 rows a K/V head are split over the keys, in one or two blocks of 16; more go in tiles.  16 sequences
     // of 2048 keys, 32/8 heads of 128, 20 rows: 41 µs split and 52 in tiles (int8), 43 and 48 (float16), 76 and 78
     // (float32); 40 rows (in four blocks): 68 and 56, 99 and 52, 134 and 86.
-    if (rows <= 32) {
+    if (rows <= (hd <= 128 ? 32 : 16)) {   // two blocks of 256 columns do not fit the registers
+        const long long steps = ((s->i[6] << s->i[4]) + STEP_WG - 1) / STEP_WG;
+        if (s->i[1] * s->i[2] > 0 && steps > ((1LL << 31) - 1) / s->i[2] / s->i[1]) {
+            lbr_set_error("paged_attention: tables of %lld sequences reach more steps than one launch takes", s->i[1]);
+            return LBR_ERR_INVALID;
+        }
         const int nr = rows <= 16 ? 1 : 2;
         if (s->i[0] == LBR_CACHE_F32) choose_split<LBR_CACHE_F32>(s, hd, nr);
         else if (s->i[0] == LBR_CACHE_F16) choose_split<LBR_CACHE_F16>(s, hd, nr);
