@@ -14,7 +14,7 @@ namespace {
 // flight.  A wavefront's 64 MFMAs a tile (head_dim 128, exact types) take 2048 cycles and the softmax of its 32 values
 // a lane about 1400 of the other unit's: two wavefronts a SIMD overlap the two.
 //
-// A small grid is multiplied by ranges of the keys (blockIdx.y), which paged_tiles_merge joins.
+// A small grid is multiplied by ranges of the keys, which paged_tiles_merge joins.
 
 constexpr int ROWS_WG = 128;
 constexpr int KS_UP = 40;           // K scales are held this many powers of two lower, q's higher
@@ -31,15 +31,16 @@ __device__ __forceinline__ int tile_keys(const PagedAttn& a, const Span& sp, int
     return sp.keys == 0 || first >= sp.count ? 0 : min(sp.start + min(last, sp.count - 1) + 1, sp.keys);
 }
 
-// (K/V head of a sequence, row tile) of a workgroup: the tiles with the most keys first; with a multiple of
-// eight heads all tiles of a head on one XCD, whose L2 then holds its keys for them.  `fold`: all workgroups are
-// there at once, two a CU; the second half then goes from the fewest keys up, beside the first's most.
-__device__ __forceinline__ void tile_of(int id, int tiles, int heads, bool fold, int& bh, int& tile) {
-    const int lanes = heads % 8 == 0 ? 8 : 1, own = heads / lanes, all = own * tiles;
+// (K/V head of a sequence, row tile, range of its keys) of a workgroup: the tiles with the most keys first; with a
+// multiple of eight heads all tiles of a head on one XCD, whose L2 then holds its keys for them.  `fold`: all
+// workgroups are there at once, two a CU; the second half then goes from the fewest keys up, beside the first's most.
+__device__ __forceinline__ void tile_of(int id, int tiles, int heads, int splits, bool fold, int& bh, int& tile, int& split) {
+    const int lanes = heads % 8 == 0 ? 8 : 1, own = heads / lanes, all = own * tiles * splits;
     int at = id / lanes;
     if (fold && at >= (all + 1) / 2) at = all - 1 - (at - (all + 1) / 2);
     bh = at % own * lanes + id % lanes;
-    tile = tiles - 1 - at / own;
+    split = at / own % splits;
+    tile = tiles - 1 - at / own / splits;
 }
 
 // K rows lie in LDS as chunks of eight columns, chunk ch of key k at place ch ^ swizzle(k): 16 keys' reads of a
@@ -48,7 +49,7 @@ template <int CH>
 __device__ __forceinline__ int swizzle(int key) { return CH == 8 ? key >> 1 & 7 : key & 15; }
 
 template <int TYPE, int HD>
-__global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void paged_tiles(PagedAttn a, int tiles, bool fold) {
+__global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void paged_tiles(PagedAttn a, int tiles, int splits, bool fold) {
     constexpr int ES = cache_elem(TYPE);
     constexpr int PL = TYPE == LBR_CACHE_F32 ? 2 : 1;
     constexpr int KT = PL == 2 ? 32 : 64;       // keys a tile
@@ -69,13 +70,12 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void paged_tiles(PagedAttn a
     const int n = lane & 31, hf = lane >> 5;
     const PagedCache& c = a.c;
     const int mask = (1 << c.shift) - 1;
-    int bh, tile;
-    tile_of(blockIdx.x, tiles, a.B * c.heads, fold, bh, tile);
+    int bh, tile, split;
+    tile_of(blockIdx.x, tiles, a.B * c.heads, splits, fold, bh, tile, split);
     const int b = bh / c.heads, h = bh % c.heads;
     const Span sp = span_of(a, b);
     const int keys = tile_keys(a, sp, tile);
     const int all = (keys + KT - 1) / KT;                       // tiles of keys
-    const int splits = gridDim.y, split = blockIdx.y;
     const int t0 = (int)((long long)all * split / splits), t1 = (int)((long long)all * (split + 1) / splits);
 
     // this lane's row
@@ -399,7 +399,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void paged_tiles(PagedAttn a
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const bool whole = splits == 1;
-    float* const part = a.parts + ((long long)split * gridDim.x + blockIdx.x) * tile_floats<HD>();
+    float* const part = a.parts + ((long long)(bh * tiles + tile) * splits + split) * tile_floats<HD>();
     if (!whole && hf == 0) {
         part[ROWS_WG * HD + wave * 32 + n] = m;
         part[ROWS_WG * HD + ROWS_WG + wave * 32 + n] = __builtin_amdgcn_ldexpf(l, 127 - vup);
@@ -426,25 +426,24 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void paged_tiles(PagedAttn a
         }
 }
 
-// Joins the ranges of the keys: one workgroup eight rows of a workgroup of paged_tiles.
-template <int HD>
-__global__ __launch_bounds__(256) void paged_tiles_merge(PagedAttn a, int tiles, int splits, bool fold) {
+// Joins the ranges of the keys: one workgroup eight rows of a workgroup of paged_tiles.  AHEAD: ranges whose loads
+// are in flight at once.
+template <int HD, int AHEAD>
+__global__ __launch_bounds__(256) void paged_tiles_merge(PagedAttn a, int tiles, int splits) {
     constexpr int LANES = HD / 4, EACH = 256 / LANES;
     const PagedCache& c = a.c;
-    int bh, tile;
-    tile_of(blockIdx.x, tiles, a.B * c.heads, fold, bh, tile);
+    const int bh = blockIdx.x / tiles, tile = blockIdx.x % tiles;
     const int b = bh / c.heads, h = bh % c.heads;
     const int r = blockIdx.y * EACH + threadIdx.x / LANES, row = tile * ROWS_WG + r, col = threadIdx.x % LANES * 4;
     if (row >= a.rows) return;
     float m = -INFINITY, l = 0.f;
     floatx4 o = {0.f, 0.f, 0.f, 0.f};
-    constexpr int AHEAD = 8;   // loads in flight
     for (int k0 = 0; k0 < splits; k0 += AHEAD) {
         float pm[AHEAD], ps[AHEAD];
         floatx4 v[AHEAD];
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
-            const float* const part = a.parts + ((long long)min(k0 + k, splits - 1) * gridDim.x + blockIdx.x) * tile_floats<HD>();
+            const float* const part = a.parts + ((long long)blockIdx.x * splits + min(k0 + k, splits - 1)) * tile_floats<HD>();
             pm[k] = part[ROWS_WG * HD + r];
             ps[k] = part[ROWS_WG * HD + ROWS_WG + r];
             v[k] = *(const floatx4*)(part + r * HD + col);
@@ -457,6 +456,15 @@ __global__ __launch_bounds__(256) void paged_tiles_merge(PagedAttn a, int tiles,
     const Span sp = span_of(a, b);
     const int token = (int)lbr_fdiv((unsigned)row, a.G_m, a.G_s), g = row - token * a.G;
     float* const to = a.out + ((long long)(b * a.H + h * a.G + g) * a.S + token) * c.hd;
+    if (a.vec && col + 4 <= c.hd) {
+        float4 v;
+        v.x = row_value(a, sp, token, o[0] * inv);
+        v.y = row_value(a, sp, token, o[1] * inv);
+        v.z = row_value(a, sp, token, o[2] * inv);
+        v.w = row_value(a, sp, token, o[3] * inv);
+        *(float4*)(to + col) = v;
+        return;
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (col + e < c.hd) to[col + e] = row_value(a, sp, token, o[e] * inv);
@@ -475,10 +483,13 @@ void launch_tiles(const Step& s, hipStream_t st) {
     const unsigned wgs = (unsigned)(tiles * s.i[1] * s.i[2]);
     if (!wgs) return;
     const unsigned lds = (unsigned)tiles_lds<TYPE, HD>();
-    const bool fold = splits == 1 && wgs <= 2u * (unsigned)lbr_device_cus();
-    hipLaunchKernelGGL((paged_tiles<TYPE, HD>), dim3(wgs, (unsigned)splits), dim3(256), lds, st, a, tiles, fold);
-    if (splits > 1)
-        hipLaunchKernelGGL((paged_tiles_merge<HD>), dim3(wgs, ROWS_WG * (HD / 4) / 256), dim3(256), 0, st, a, tiles, splits, fold);
+    const bool fold = wgs * (unsigned)splits <= 2u * (unsigned)lbr_device_cus();
+    hipLaunchKernelGGL((paged_tiles<TYPE, HD>), dim3(wgs * (unsigned)splits), dim3(256), lds, st, a, tiles, splits, fold);
+    const dim3 joins(wgs, ROWS_WG * (HD / 4) / 256);
+    if (splits == 2)
+        hipLaunchKernelGGL((paged_tiles_merge<HD, 2>), joins, dim3(256), 0, st, a, tiles, splits);
+    else if (splits > 2)
+        hipLaunchKernelGGL((paged_tiles_merge<HD, 8>), joins, dim3(256), 0, st, a, tiles, splits);
 }
 
 template <int TYPE>
