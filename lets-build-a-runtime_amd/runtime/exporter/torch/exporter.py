@@ -7,17 +7,20 @@ weight constants according to the export signature, every ``call_function``
 node is mapped by the ATen handler registry, and the output node names the
 graph outputs.  Tensor names are the fx node names, so node and tensor
 naming — and with it node ids and planner order — match the reference for
-the same model and torch version.
+the same model and torch version.  Buffers that the paged-cache ops (``lbr::…``) take
+become states of the graph, which keep their contents from run to run.
 """
 
 from __future__ import annotations
+
+import inspect
 
 import torch
 import torch.nn as nn
 from torch.export.graph_signature import InputKind
 
 from ...ir import Graph
-from .handlers import ATEN_HANDLERS
+from .handlers import ATEN_HANDLERS, cache_argument
 
 
 def export_pytorch(model: nn.Module, example_inputs: tuple,
@@ -43,6 +46,13 @@ def _export_core(model, example_inputs, dynamic_dims=None, example_kwargs=None) 
             dim = torch.export.Dim(sym, min=1)
             for input_name, idx in specs:
                 torch_dynamic.setdefault(input_name, {})[idx] = dim
+        # torch wants every argument named: the others are static
+        given = list(inspect.signature(model.forward).parameters.values())[:len(example_inputs)]
+        for p in given:
+            if p.kind not in (p.VAR_POSITIONAL, p.VAR_KEYWORD):
+                torch_dynamic.setdefault(p.name, None)
+        for name in example_kwargs or {}:
+            torch_dynamic.setdefault(name, None)
         extra = {"strict": False, "prefer_deferred_runtime_asserts_over_guards": True}
 
     exported = torch.export.export(model, example_inputs, kwargs=example_kwargs or {},
@@ -79,6 +89,8 @@ def _process_placeholders(exported, graph: Graph, node_map: dict[str, str]) -> N
         kinds[spec.arg.name] = spec.kind
         if spec.target is not None:
             targets[spec.arg.name] = spec.target
+    caches = {a.name for fx in exported.graph_module.graph.nodes if fx.op == "call_function"
+              if (a := cache_argument(fx)) is not None}
     for fx in exported.graph_module.graph.nodes:
         if fx.op != "placeholder":
             continue
@@ -89,7 +101,8 @@ def _process_placeholders(exported, graph: Graph, node_map: dict[str, str]) -> N
         if kind == InputKind.USER_INPUT:
             graph.inputs.append(fx.name)
         elif kind in (InputKind.PARAMETER, InputKind.BUFFER):
-            graph.constants.append(fx.name)
+            state = fx.name in caches
+            (graph.states if state else graph.constants).append(fx.name)
             key = targets[fx.name]
             if key in exported.state_dict:
                 info.buffer = exported.state_dict[key].numpy(force=True)
@@ -97,6 +110,8 @@ def _process_placeholders(exported, graph: Graph, node_map: dict[str, str]) -> N
                 info.buffer = exported.constants[key].numpy(force=True)
             else:
                 raise ValueError(f"Weight/buffer '{key}' not found in state_dict or constants")
+            if state:   # a copy: the model's own runs change the buffer; none for zeros, a state's default
+                info.buffer = info.buffer.copy() if info.buffer.any() else None
 
 
 def _process_compute_nodes(exported, graph: Graph, node_map: dict[str, str], symbol_map: dict[str, str]) -> None:
@@ -104,10 +119,10 @@ def _process_compute_nodes(exported, graph: Graph, node_map: dict[str, str], sym
         if fx.op != "call_function":
             continue
         val = fx.meta.get("val")
-        if val is None:
+        if val is None and cache_argument(fx) is None:
             continue  # deferred runtime assertions
-        if not isinstance(val, torch.Tensor) and not (isinstance(val, tuple) and val
-                                                      and isinstance(val[0], torch.Tensor)):
+        if val is not None and not isinstance(val, torch.Tensor) and not (isinstance(val, tuple) and val
+                                                                          and isinstance(val[0], torch.Tensor)):
             continue  # SymInt arithmetic, sym_size
         handler = ATEN_HANDLERS.get(fx.target)
         if handler is None:

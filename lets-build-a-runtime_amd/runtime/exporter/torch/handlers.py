@@ -7,7 +7,7 @@ exactly two axes, split + getitem → SLICE with a byte offset, SDPA →
 ATTENTION with causal / GQA group_size), same tensor naming (fx node names
 plus ``_weight_t`` / ``_mm`` / ``_sum`` suffixes).  Note: ``aten.gelu`` maps
 to the tanh-approximation GELU whatever its ``approximate`` argument, as in
-the reference (handlers.py:605).
+the reference (handlers.py:605).  The paged-cache ops (``lbr::…``, paged_ops.py) have no counterpart there.
 """
 
 from __future__ import annotations
@@ -20,6 +20,8 @@ import numpy as np
 import torch
 
 from ...ir import Graph, OpType
+from ...paged import CacheLayout
+from . import paged_ops  # noqa: F401 — registers the lbr ops
 
 OpHandler = Callable[[object, Graph, dict, dict], None]
 
@@ -350,7 +352,53 @@ def _handle_cat(fx, graph, node_map, symbol_map):
     _emit(fx, graph, node_map, OpType.CAT, [node_map[t.name] for t in tensors], {"dim": dim})
 
 
+def _op_args(fx) -> dict:
+    """A custom op's arguments by name, defaults filled in."""
+    args = {a.name: a.default_value for a in fx.target._schema.arguments if a.has_default_value()}
+    args.update(zip((a.name for a in fx.target._schema.arguments), fx.args))
+    return {**args, **fx.kwargs}
+
+
+def cache_argument(fx):
+    """The fx node that a paged-cache op takes its cache from, or None."""
+    return _op_args(fx)["cache"] if fx.target in CACHE_OPS else None
+
+
+def _cache_op(op: OpType, names: tuple[str, ...], layout: Callable, attrs: tuple[str, ...] = ()) -> OpHandler:
+    """An op that reads a cache: tensors by name, the layout, and attributes that are not None."""
+    def handler(fx, graph, node_map, symbol_map):
+        a = _op_args(fx)
+        more = {k: a[k] for k in attrs if a[k] is not None}
+        _emit(fx, graph, node_map, op, [node_map[a[n].name] for n in names], {**layout(a).attrs, **more})
+    return handler
+
+
+def _handle_cache_write(fx, graph, node_map, symbol_map):
+    """cache_write changes a buffer: the buffer's later uses take the written tensor, which is the same memory."""
+    a = _op_args(fx)
+    cache = node_map[a["cache"].name]
+    if graph.state_of(cache) is None:
+        raise ValueError(f"cache_write: '{a['cache'].name}' is not a buffer of the model")
+    heads, hd = (a["k"].meta["val"].shape[d] for d in (1, 3))
+    lay = CacheLayout(int(heads), int(hd), a["page_size"], a["cache_type"])
+    graph.add_tensor(fx.name, graph.tensors[cache].shape, "uint8")
+    graph.add_node(OpType.CACHE_WRITE,
+                   [cache, *(node_map[a[n].name] for n in ("k", "v", "page_table", "start", "count"))],
+                   fx.name, lay.attrs)
+    node_map[a["cache"].name] = fx.name
+
+
+def _handle_verify_draft(fx, graph, node_map, symbol_map):
+    a = _op_args(fx)
+    _emit(fx, graph, node_map, OpType.VERIFY_DRAFT,
+          [node_map[a[n].name] for n in ("target", "draft", "tokens", "uniforms", "count")])
+
+
 aten = torch.ops.aten
+lbr = torch.ops.lbr
+
+# the ops over a cache, which the exporter makes a state
+CACHE_OPS = (lbr.cache_write.default, lbr.cache_read.default, lbr.paged_attention.default)
 
 ATEN_HANDLERS: dict[object, OpHandler] = {
     aten.relu.default: _simple(OpType.RELU),
@@ -411,4 +459,13 @@ ATEN_HANDLERS: dict[object, OpHandler] = {
     aten.dropout.default: _handle_noop,
     aten.alias.default: _handle_noop,
     aten._assert_tensor_metadata.default: _handle_assert_metadata,
+    lbr.cache_write.default: _handle_cache_write,
+    lbr.cache_read.default: _cache_op(
+        OpType.CACHE_READ, ("cache", "page_table", "start", "count"),
+        lambda a: CacheLayout(a["kv_heads"], a["head_dim"], a["page_size"], a["cache_type"]), ("length",)),
+    lbr.paged_attention.default: _cache_op(
+        OpType.PAGED_ATTENTION, ("q", "cache", "page_table", "start", "count"),
+        lambda a: CacheLayout(a["kv_heads"], int(a["q"].meta["val"].shape[3]), a["page_size"], a["cache_type"]),
+        ("scale",)),
+    lbr.verify_draft.default: _handle_verify_draft,
 }

@@ -58,6 +58,62 @@ class CausalGeluBlock(nn.Module):
         return x + self.ffn2(F.gelu(self.ffn1(self.ln2(x)), approximate="tanh"))
 
 
+class CachedGeluBlock(CausalGeluBlock):
+    """CausalGeluBlock that continues its sequences: x holds the next chunk of each, ``start`` how many of its
+    positions the paged cache holds already, ``count`` how many rows of the chunk are real, ``page_table``
+    the pages of each sequence.  The outputs of a sequence's chunks, one behind the other, are those of
+    CausalGeluBlock over the whole."""
+
+    def __init__(self, d_model: int, n_heads: int, pages: int, page_size: int, cache_type: str = "float16",
+                 ffn_mult: int = 4, kv_heads: int | None = None) -> None:
+        from runtime.exporter.torch.paged_ops import CacheLayout   # and the ops themselves
+        super().__init__(d_model, n_heads, ffn_mult)
+        self.layout = CacheLayout(kv_heads or n_heads, self.d_k, page_size, cache_type)
+        if kv_heads:
+            self.wk, self.wv = (nn.Linear(d_model, kv_heads * self.d_k) for _ in range(2))
+        self.register_buffer("cache", torch.zeros(self.layout.shape(pages), dtype=torch.uint8))
+
+    def forward(self, x, page_table, start, count):
+        B, S, D = x.shape
+        lay = self.layout
+        h = self.ln1(x)
+        q = self.wq(h).reshape(B, S, self.n_heads, self.d_k).permute(0, 2, 1, 3)
+        k = self.wk(h).reshape(B, S, lay.kv_heads, self.d_k).permute(0, 2, 1, 3)
+        v = self.wv(h).reshape(B, S, lay.kv_heads, self.d_k).permute(0, 2, 1, 3)
+        torch.ops.lbr.cache_write(self.cache, k, v, page_table, start, count, lay.page_size, lay.cache_type)
+        a = torch.ops.lbr.paged_attention(q, self.cache, page_table, start, count, lay.kv_heads, lay.page_size,
+                                          lay.cache_type)
+        x = x + self.wo(a.permute(0, 2, 1, 3).reshape(B, S, D))
+        return x + self.ffn2(F.gelu(self.ffn1(self.ln2(x)), approximate="tanh"))
+
+
+class CachedLM(nn.Module):
+    """A language model of CachedGeluBlocks with learned positions and tied embeddings: the probabilities
+    behind each token of a chunk, for generation with a paged cache (``generate``)."""
+
+    def __init__(self, vocab: int, n_layer: int, n_head: int, n_embd: int, n_positions: int, pages: int, page_size: int,
+                 cache_type: str = "float16", kv_heads: int | None = None) -> None:
+        super().__init__()
+        self.wte = nn.Embedding(vocab, n_embd)
+        self.wpe = nn.Embedding(n_positions, n_embd)
+        self.h = nn.ModuleList([CachedGeluBlock(n_embd, n_head, pages, page_size, cache_type, kv_heads=kv_heads)
+                                for _ in range(n_layer)])
+        self.ln_f = nn.LayerNorm(n_embd)
+
+    def forward(self, ids, positions, page_table, start, count):
+        x = self.wte(ids) + self.wpe(positions)
+        for block in self.h:
+            x = block(x, page_table, start, count)
+        return torch.softmax(F.linear(self.ln_f(x), self.wte.weight), -1)
+
+
+class DraftCheck(nn.Module):
+    """Which drafted tokens of a chunk stand, and the token behind them (torch.ops.lbr.verify_draft)."""
+
+    def forward(self, target, draft, tokens, uniforms, count):
+        return torch.ops.lbr.verify_draft(target, draft, tokens, uniforms, count)
+
+
 class GPT2Body(nn.Module):
     """GPT-2 transformer body: learned position embeddings + blocks + ln_f."""
 
@@ -211,6 +267,117 @@ def export_workload(key: str, seed: int = 0, seq_len: int | None = None, batch: 
     x = w.input(seed, seq_len, batch)
     graph = export_model(model, (torch.from_numpy(x),))
     return model, x, graph
+
+
+class Generator:
+    """Sequences continued by a CachedLM, and by a smaller one that drafts: sessions over the models' caches,
+    one plan for each chunk length.  Every sequence has its own pages, in order of its positions."""
+
+    def __init__(self, model: CachedLM, batch: int, draft: CachedLM | None = None, drafts: int = 3) -> None:
+        lay = model.h[0].layout
+        self.batch, self.drafts = batch, drafts if draft is not None else 0
+        self.wide = model.h[0].cache.shape[0] // batch
+        if self.wide < 1:
+            raise ValueError(f"a cache of {model.h[0].cache.shape[0]} pages is too small for {batch} sequences")
+        self.room = min(self.wide * lay.page_size, model.wpe.num_embeddings)
+        self.table = np.arange(batch * self.wide, dtype=np.int32).reshape(batch, self.wide)
+        self.target = self._session(model)
+        self.draft = None if draft is None else self._session(draft)
+        if draft is not None and (draft.h[0].cache.shape[0] < batch * self.wide
+                                  or draft.h[0].layout.page_size != lay.page_size
+                                  or draft.wte.num_embeddings != model.wte.num_embeddings
+                                  or draft.wpe.num_embeddings < self.room):
+            raise ValueError("the drafting model needs the target's vocabulary, positions and pages")
+        if draft is not None:
+            d, vocab = self.drafts, model.wte.num_embeddings
+            self.check = self._create(DraftCheck(), (
+                torch.zeros(batch, d + 1, vocab), torch.zeros(batch, d, vocab), torch.zeros(batch, d, dtype=torch.int64),
+                torch.zeros(batch, d + 1), torch.zeros(batch, dtype=torch.int32)))
+
+    def _create(self, model, example, dynamic=None, **bindings):
+        from runtime.exporter import export_model
+        from runtime.session import Session
+        s = Session(export_model(model, example, dynamic))
+        s.create(bindings=bindings or None)
+        return s
+
+    def _session(self, model):
+        # tensors of their own: one given twice would be one input
+        ids, positions = (torch.zeros(self.batch, 2, dtype=torch.int64) for _ in range(2))
+        start, count = (torch.zeros(self.batch, dtype=torch.int32) for _ in range(2))
+        return self._create(model, (ids, positions, torch.from_numpy(self.table), start, count),
+                            {"L": [("ids", 1), ("positions", 1)]}, L=1)
+
+    def step(self, session, ids, start, count):
+        """Probabilities [batch, L, vocab] behind each of the chunks' tokens, which go into the cache."""
+        length = ids.shape[1]
+        session.rebind({"L": length})
+        positions = np.minimum(start[:, None].astype(np.int64) + np.arange(length), self.room - 1)
+        out = session.run({"ids": ids, "positions": positions, "page_table": self.table,
+                           "start": start.astype(np.int32), "count": count.astype(np.int32)})
+        return next(iter(out.values()))
+
+    def generate(self, prompts: list, tokens: int, seed: int = 0) -> list:
+        """`tokens` more tokens for each prompt, drawn from the target's probabilities."""
+        if len(prompts) != self.batch or not all(len(p) for p in prompts):
+            raise ValueError(f"expected {self.batch} prompts of at least one token")
+        if max(map(len, prompts)) + tokens + self.drafts > self.room:
+            raise ValueError(f"{max(map(len, prompts))} + {tokens} tokens and {self.drafts} drafted ones do not fit "
+                             f"{self.room} positions")
+        if tokens < 1:
+            return [[] for _ in prompts]
+        r = np.random.default_rng(seed)
+        length = np.array([len(p) for p in prompts])
+        ids = np.zeros((self.batch, length.max()), np.int64)
+        for b, p in enumerate(prompts):
+            ids[b, :len(p)] = p
+        zero = np.zeros(self.batch, np.int64)
+        p = self.step(self.target, ids, zero, length)
+        if self.draft is not None:
+            self.step(self.draft, ids, zero, length)
+        new = [[t] for t in _drawn(p[np.arange(self.batch), length - 1], r)]
+        held = length.copy()   # positions in the target's cache; the newest token is behind them
+        before = np.array([q[-1] for q in prompts])   # the token at position held - 1
+        while min(map(len, new)) < tokens:
+            newest = np.array([n[-1] for n in new])
+            live = np.array([len(n) < tokens for n in new])
+            if self.draft is None:
+                p = self.step(self.target, newest[:, None], held, live.astype(np.int64))
+                for b, t in enumerate(_drawn(p[:, 0], r)):
+                    if live[b]:
+                        new[b].append(t)
+                held += live
+                continue
+            # the draft's cache may lack position held - 1, the last of its own drafts: it is written again
+            drafted, q = [], []
+            p = self.step(self.draft, np.stack([before, newest], 1), held - 1, 2 * live)[:, 1]
+            for i in range(self.drafts):
+                q.append(p)
+                drafted.append(_drawn(p, r, live))
+                if i + 1 < self.drafts:
+                    p = self.step(self.draft, np.array(drafted[-1])[:, None], held + 1 + i, live.astype(np.int64))[:, 0]
+            drafted = np.array(drafted).T
+            p = self.step(self.target, np.concatenate([newest[:, None], drafted], 1), held, (self.drafts + 1) * live)
+            out = next(iter(self.check.run({
+                "target": p, "draft": np.stack(q, 1), "tokens": drafted,
+                "uniforms": r.random((self.batch, self.drafts + 1), np.float32),
+                "count": (self.drafts * live).astype(np.int32)}).values()))
+            for b in np.flatnonzero(live):
+                stand = [int(t) for t in out[b] if t >= 0]
+                if not stand:
+                    raise RuntimeError(f"sequence {b}: the model's probabilities are none")
+                before[b] = stand[-2] if len(stand) > 1 else newest[b]
+                new[b] += stand
+                held[b] += len(stand)
+        return [n[:tokens] for n in new]
+
+
+def _drawn(p: np.ndarray, r: np.random.Generator, live=None) -> list:
+    """A token for each row of probabilities (0 for rows that are not live)."""
+    u = r.random(len(p))
+    run = np.cumsum(p, -1, dtype=np.float64)
+    at = [min(int(np.searchsorted(run[b], u[b] * run[b, -1], "right")), p.shape[1] - 1) for b in range(len(p))]
+    return at if live is None else [t if alive else 0 for t, alive in zip(at, live)]
 
 
 def reference_forward(model: nn.Module, x: np.ndarray, dtype=torch.float64) -> np.ndarray:
