@@ -199,6 +199,7 @@ def _compute_lifetimes(graph: Graph, order: list[Node],
                        config: PlannerConfig | None = None) -> tuple[dict[str, Lifetime], dict[str, str]]:
     config = config or PlannerConfig()
     external = graph.external
+    kept = {_resolve_alias(t, graph) for t in graph.outputs}   # nothing takes their place in the arena
     memory_root: dict[str, str] = {}
 
     def root_of(name: str) -> str:
@@ -232,12 +233,14 @@ def _compute_lifetimes(graph: Graph, order: list[Node],
                 continue
         if config.enable_inplace and op_def is not None and op_def.inplace and node.inputs:
             src = _resolve_alias(node.inputs[0], graph)
-            if (src not in external and seen_uses[src] == total_uses[src]
+            if (src not in external and src not in kept and seen_uses[src] == total_uses[src]
                     and _tensor_size(graph, src) == _tensor_size(graph, node.output)):
                 memory_root[node.output] = root_of(src)
                 continue
         born[node.output] = step
 
+    for t in kept:
+        dies[root_of(t)] = len(order) - 1
     lifetimes = {name: Lifetime(name, _tensor_size(graph, name), b, dies.get(name, b)) for name, b in born.items()}
     return lifetimes, memory_root
 

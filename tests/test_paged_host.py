@@ -305,3 +305,26 @@ def test_reference_pack_is_the_layout():
         assert k[slot * 32 + d] == p.y[page, h, 0, slot, d]
         assert v[(slot // 8 * 32 + d) * 8 + slot % 8] == p.y[page, h, 1, slot, d]
         assert s[slot] == p.s[page, h, 0, slot] and s[32 + slot] == p.s[page, h, 1, slot]
+
+
+@pytest.mark.parametrize("read", [1, 5, 6, 40])
+def test_plan_keeps_every_output(read):
+    """An output that no later node takes stays where it is until the end, whatever is computed behind it."""
+    g = step_graph(batch=1, heads=2, chunk=read, read=read)
+    mem = plan(g)
+    assert not run_validators(Phase.POST_PLAN, mem)
+    span = {n: (mem.offsets[n], mem.offsets[n] + 4 * int(np.prod(g.tensors[n].shape))) for n in g.outputs}
+    (a0, a1), (b0, b1) = span.values()
+    assert a1 <= b0 or b1 <= a0
+
+
+def test_plan_overwrites_no_output_in_place():
+    g = Graph()
+    _tensor(g, "x", (8, 8))
+    _tensor(g, "y", (8, 8), role="outputs")
+    _tensor(g, "z", (8, 8), role="outputs")
+    g.add_node(OpType.EXP, ["x"], "y")
+    g.add_node(OpType.RELU, ["y"], "z")
+    mem = plan(g)
+    assert not run_validators(Phase.POST_PLAN, mem)
+    assert mem.offsets["y"] != mem.offsets["z"]
