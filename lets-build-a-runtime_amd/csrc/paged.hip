@@ -344,9 +344,9 @@ step_fn read_for(int hd) {
     return hd <= 64 ? launch_read<TYPE, 16> : hd <= 128 ? launch_read<TYPE, 32> : launch_read<TYPE, 64>;
 }
 
-// Whether the wavefronts of a launch, one for each eight rows of a head, can be counted in its grid.
+// Whether a launch holds a wavefront for each eight rows of a head: its threads are counted in 32 bits.
 bool units_fit(const Step& s, const char* what) {
-    const long long groups = (s.i[7] + 14) / 8, most = (1LL << 31) - 1;
+    const long long groups = (s.i[7] + 14) / 8, most = (1LL << 26) - 4;
     if (s.i[1] <= most / s.i[2] && (s.i[1] == 0 || groups <= most / (s.i[1] * s.i[2]))) return true;
     lbr_set_error("%s: %lld sequences of %lld rows are more than one launch takes", what, s.i[1], s.i[7]);
     return false;
@@ -371,7 +371,7 @@ int decode_paged_common(const OpNode* n, Step* s, int cache, int first, long lon
         return LBR_ERR_INVALID;
     }
     const long long head_bytes = (long long)page * (2LL * ((hd + 15) / 16 * 16) * cache_elem(type) + 8);
-    if (heads > ((1LL << 31) - 1) / head_bytes || x[4] < 1 || x[5] < 1 || (long long)x[5] * page >= (1LL << 31)) {
+    if (heads > ((1LL << 31) - 1) / head_bytes || x[4] < 1 || x[5] < 1 || (long long)x[5] * page > (1LL << 30)) {
         lbr_set_error("cache of %d pages of %d heads, tables of %d pages of %d positions", x[4], heads, x[5], page);
         return LBR_ERR_INVALID;
     }

@@ -40,7 +40,7 @@ struct PagedAttn {
     bool vec;                 // rows of q and out on 16-byte boundaries
 };
 
-// A sequence's rows and keys: count of rows 0 .. S, keys 0 .. the table's end (0 where start is negative).
+// A sequence's rows and keys: count of rows 0 .. S, keys 0 .. the table's end, at most 2^30 (0 where start is negative).
 struct Span {
     int start, count, keys;
 };
@@ -53,10 +53,15 @@ __device__ __forceinline__ Span span_of(const PagedAttn& a, int b) {
     return s;
 }
 
+// The last key of a row, −1 for a row that has none; a row that reaches past the table ends with the table.
+__device__ __forceinline__ int last_key(const Span& s, int token) {
+    return token < s.count ? (int)min((long long)s.start + token, (long long)s.keys - 1) : -1;
+}
+
 // A row's result from its sum: zeros behind the sequence's rows, NaN where the table does not reach.
 __device__ __forceinline__ float row_value(const PagedAttn& a, const Span& s, int token, float v) {
     if (token >= s.count) return 0.f;
-    return s.start < 0 || s.start + token >= ((long long)a.c.wide << a.c.shift) ? __uint_as_float(0x7fc00000u) : v;
+    return s.start < 0 || (long long)s.start + token >= ((long long)a.c.wide << a.c.shift) ? __uint_as_float(0x7fc00000u) : v;
 }
 
 // ---------------------------------------------------------------- fp16 operands

@@ -281,7 +281,7 @@ __global__ __launch_bounds__(256, (split_occupancy<TYPE, HD, NR>())) void paged_
         for (int t = 0; t < NR; ++t) {
             const int r = 16 * t + n, token = (int)lbr_fdiv((unsigned)min(r, a.rows - 1), a.G_m, a.G_s);
             qs[t] = q_scale[r];
-            last[t] = r < a.rows && token < sp.count ? sp.start + token : -1;
+            last[t] = r < a.rows ? last_key(sp, token) : -1;
         }
 
         floatx4 o[NR][ND];
@@ -681,6 +681,11 @@ int decode_paged_attention(const OpNode* n, Step* s) {
         lbr_set_error("paged_attention: %lld rows are more than one launch takes", node_total(n) / d[3]);
         return LBR_ERR_INVALID;
     }
+    // a launch's threads are counted in 32 bits, 256 a workgroup
+    if (s->i[1] * s->i[2] >= 1LL << 24) {
+        lbr_set_error("paged_attention: %lld sequences of %lld heads are more than one launch takes", s->i[1], s->i[2]);
+        return LBR_ERR_INVALID;
+    }
     const int hd = (int)s->i[3];
     const long long rows = s->i[8] / s->i[2] * s->i[7];
     s->i[9] = hd % 4 == 0 && lbr_aligned(s->in[4], 16) && lbr_aligned(s->out, 16);
@@ -702,7 +707,7 @@ int decode_paged_attention(const OpNode* n, Step* s) {
         return LBR_OK;
     }
     // grid: row tiles of all K/V heads
-    if (paged_row_tiles(*s) > ((1LL << 31) - 1) / (s->i[2] * (s->i[1] > 0 ? s->i[1] : 1))) {
+    if (paged_row_tiles(*s) >= (1LL << 24) / (s->i[2] * (s->i[1] > 0 ? s->i[1] : 1))) {
         lbr_set_error("paged_attention: %lld rows are more than one launch takes", node_total(n) / d[3]);
         return LBR_ERR_INVALID;
     }

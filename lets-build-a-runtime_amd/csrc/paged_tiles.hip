@@ -28,7 +28,7 @@ constexpr int tile_floats() { return ROWS_WG * (HD + 2); }
 __device__ __forceinline__ int tile_keys(const PagedAttn& a, const Span& sp, int tile) {
     const int first = (int)lbr_fdiv((unsigned)(tile * ROWS_WG), a.G_m, a.G_s);
     const int last = (int)lbr_fdiv((unsigned)min(tile * ROWS_WG + ROWS_WG, a.rows) - 1u, a.G_m, a.G_s);
-    return sp.keys == 0 || first >= sp.count ? 0 : min(sp.start + min(last, sp.count - 1) + 1, sp.keys);
+    return sp.keys == 0 || first >= sp.count ? 0 : last_key(sp, min(last, sp.count - 1)) + 1;
 }
 
 // (K/V head of a sequence, row tile, range of its keys) of a workgroup: the tiles with the most keys first; with a
@@ -84,7 +84,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void paged_tiles(PagedAttn a
     const int token = (int)lbr_fdiv((unsigned)rc, a.G_m, a.G_s), g = rc - token * a.G;
     const long long qat = ((long long)(b * a.H + h * a.G + g) * a.S + token) * c.hd;
     const bool mine = row < a.rows && token < sp.count;
-    const int last = mine ? sp.start + token : -1;             // its last key
+    const int last = mine ? last_key(sp, token) : -1;          // its last key
     int wave_last = last;
     for (int o = 16; o; o >>= 1) wave_last = max(wave_last, __shfl_xor(wave_last, o, 64));
     wave_last = __builtin_amdgcn_readfirstlane(wave_last);   // the halves hold the same rows

@@ -157,8 +157,8 @@ def check_op(op: str, shapes: list[tuple], dtypes: list[str], attrs: dict, out_s
             raise ValueError(f"{op}: pages of the cache have {by['cache'][1]} bytes, {lay} has {lay.page_bytes}")
         if by["cache"][0] < 1 or by["page_table"][1] < 1:
             raise ValueError(f"{op}: the cache and the page table need a page")
-        if by["page_table"][1] * lay.page_size >= 2**31:
-            raise ValueError(f"{op}: a table of {by['page_table'][1]} pages reaches positions past 2^31")
+        if by["page_table"][1] * lay.page_size > 2**30:
+            raise ValueError(f"{op}: a table of {by['page_table'][1]} pages reaches positions past 2^30")
         batch = by["page_table"][0]
         same("start", (batch,))
         same("count", (batch,))
