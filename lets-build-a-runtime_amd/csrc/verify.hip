@@ -10,6 +10,8 @@
 // wavefront find n for itself (its loads of tokens, numbers and probabilities, one vote) and sum 1024 entries of
 // r; a second, one wavefront a sequence, finds the part in which the running sum passes and goes through that
 // part's entries alone again, 16 in a row a lane.
+//
+// 64 sequences of five drafts, 151 936 entries: 19 µs (78 MB); one of four, 50 257: 9, two chains of loads and launches.
 #include "lbr_device.h"
 
 namespace {

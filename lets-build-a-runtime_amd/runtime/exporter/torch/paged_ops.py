@@ -7,7 +7,8 @@
 
 ``cache`` is a uint8 buffer of the model (``register_buffer``) of ``CacheLayout.shape(pages)``, which
 ``cache_write`` changes in place; the exporter makes it a state of the graph.  What the ops do, and the cache's
-bytes, is said in runtime/paged.py.  Called outside an exported graph they run here, in plain torch and 64 bits, on any
+bytes, is said in runtime/paged.py.  A cache is not read ahead of a write in one forward: nothing in a graph
+would order the two (the graph's validation says so).  Called outside an exported graph they run here, in plain torch and 64 bits, on any
 device: for a model's reference, not for speed.
 """
 

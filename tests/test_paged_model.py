@@ -13,6 +13,8 @@ from runtime.ops import resolve_graph
 from runtime.paged import CACHE_TYPES, CacheLayout
 from runtime.passes.passes import run_pipeline
 from runtime.planner import plan
+from runtime.validation import Phase, run_validators
+from runtime.validation.core import ValidationError
 
 lbr = torch.ops.lbr
 
@@ -161,24 +163,40 @@ def test_export_of_any_chunk_length(tmp_path):
     assert Graph.load(tmp_path / "g.json").states == ["b_cache"]
 
 
-def test_export_reads_what_was_written_before():
-    class Both(torch.nn.Module):
-        def __init__(self):
-            super().__init__()
-            self.register_buffer("cache", torch.zeros(CacheLayout(2, 24, 16).shape(4), dtype=torch.uint8))
+class Twice(torch.nn.Module):
+    """Two writes of a cache, attention behind them; `before`: a reading ahead of them."""
 
-        def forward(self, k, table, start, count):
-            before = lbr.cache_read(self.cache, table, start, count, 5, 2, 24, 16, "float32")
-            lbr.cache_write(self.cache, k, k, table, start, count, 16, "float32")
-            lbr.cache_write(self.cache, k + 1, k, table, start, count, 16, "float32")
-            return before, lbr.paged_attention(k, self.cache, table, start, count, 2, 16, "float32", scale=0.25)
+    def __init__(self, before):
+        super().__init__()
+        self.before = before
+        self.register_buffer("cache", torch.zeros(CacheLayout(2, 24, 16).shape(4), dtype=torch.uint8))
 
-    g = export_model(Both(), (torch.zeros(2, 2, 5, 24), torch.zeros(2, 2, dtype=torch.int32),
-                              *(torch.zeros(2, dtype=torch.int32) for _ in range(2))))
-    read, first, _, second, attend = list(g)
-    assert read.inputs[0] == first.inputs[0] == "b_cache" and second.inputs[0] == first.output
+    def forward(self, k, table, start, count):
+        out = [lbr.cache_read(self.cache, table, start, count, 5, 2, 24, 16, "float32")] if self.before else []
+        lbr.cache_write(self.cache, k, k, table, start, count, 16, "float32")
+        lbr.cache_write(self.cache, k + 1, k, table, start, count, 16, "float32")
+        return *out, lbr.paged_attention(k, self.cache, table, start, count, 2, 16, "float32", scale=0.25)
+
+
+def export_twice(before):
+    return export_model(Twice(before), (torch.zeros(2, 2, 5, 24), torch.zeros(2, 2, dtype=torch.int32),
+                                        *(torch.zeros(2, dtype=torch.int32) for _ in range(2))))
+
+
+def test_export_reads_what_was_written_last():
+    g = export_twice(False)
+    first, second = (n for n in g if n.op == OpType.CACHE_WRITE)
+    attend, = (n for n in g if n.op == OpType.PAGED_ATTENTION)
+    assert first.inputs[0] == "b_cache" and second.inputs[0] == first.output
     assert attend.inputs[1] == second.output and attend.attrs["scale"] == 0.25
+    assert not run_validators(Phase.POST_OPTIMIZE, g)
     plan(g)
+
+
+def test_a_reading_ahead_of_a_write_is_refused():
+    """Nothing in a graph orders the two."""
+    with pytest.raises(ValidationError, match="uses the value before"):
+        run_validators(Phase.POST_OPTIMIZE, export_twice(True))
 
 
 def test_export_refuses_a_cache_that_is_an_input():
