@@ -137,8 +137,9 @@ class DeviceStates:
 
 class DeviceArray:
     """A plan's device buffer for other libraries to look at without a copy
-    (``torch.as_tensor(array, device="cuda")``); it keeps the executor alive.  The library's stream
-    writes it: synchronise, or order another stream behind it with ``signal_stream``, before a read."""
+    (``torch.as_tensor(array, device="cuda")``); it keeps the executor alive, but not its memory behind a
+    ``close``, the session's or that of a plan which left its cache.  The library's stream writes it:
+    synchronise, or order another stream behind it with ``signal_stream``, before a read."""
 
     def __init__(self, owner: "CompiledExecutor", address: int, shape: tuple[int, ...], dtype: str) -> None:
         self.owner = owner

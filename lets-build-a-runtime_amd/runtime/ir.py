@@ -292,7 +292,7 @@ class Graph:
         manifest: dict[str, dict] = {}
         blobs: list[bytes] = []
         offset = 0
-        for name in self.constants:
+        for name in self.constants + self.states:   # a state's buffer is what it holds at first
             buf = self.tensors[name].buffer
             if buf is None:
                 continue

@@ -328,3 +328,11 @@ def test_plan_overwrites_no_output_in_place():
     mem = plan(g)
     assert not run_validators(Phase.POST_PLAN, mem)
     assert mem.offsets["y"] != mem.offsets["z"]
+
+
+def test_graph_file_keeps_what_a_state_holds_at_first(tmp_path):
+    g = step_graph()
+    r = np.random.default_rng(0)
+    g.tensors["cache"].buffer = r.integers(0, 256, g.tensors["cache"].shape, dtype=np.uint8)
+    g.save(tmp_path / "g")
+    np.testing.assert_array_equal(Graph.load(tmp_path / "g").tensors["cache"].buffer, g.tensors["cache"].buffer)
