@@ -41,8 +41,8 @@ The ops (graph nodes; every index tensor int32):
   running sum, in 64 bits, passes uniforms[b, D] times the whole).  Output: int64 ``[B, D + 1]``,
   the n tokens, the drawn one, then -1.  A row without a probability above zero gives -1.
 
-counts are taken as 0 .. S (``length``, D).  Positions a table does not reach, and pages that the cache
-does not have, read as NaN.
+counts are taken as 0 .. S (``length``, D).  A table's row reaches 2^30 positions at most.  Positions a
+table does not reach, and pages that the cache does not have, read as NaN.
 """
 
 from __future__ import annotations
