@@ -1,6 +1,7 @@
 // paged_tiles.hip — attention over the paged cache: chunks of more than 32 rows a K/V head.
 #include "paged_attention.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -527,12 +528,17 @@ hipError_t raise_lds_of() {
 
 int paged_row_tiles(const Step& s) { return (int)((s.i[8] / s.i[2] * s.i[7] + ROWS_WG - 1) / ROWS_WG); }
 
-// Enough for two workgroups a CU, none shorter than four tiles of keys at the table's full length.
+// Ranges of the keys for a small grid: up to two workgroups a CU where each keeps two tiles of keys at the table's full
+// length, up to one a CU where each keeps one.  64 tokens behind 1000, 8 heads of 128, float16: 49.9 µs in one range, 23.3
+// with four tiles a range, 19.0 with two, 15.1 with one (136 workgroups); 512 tokens, 12 heads of 64: 23.0, 18.4, 16.3 and
+// 19.8 (384); 3 × 77 behind 2000, 5 heads of 80, int8: 102, 28.2, 26.6, 30.2 (510), and 24.9 by this rule (255).
 int paged_tiles_splits(const Step& s) {
     const long long cus = lbr_device_cus() > 0 ? lbr_device_cus() : 256;
-    const long long wgs = paged_row_tiles(s) * s.i[1] * s.i[2], keys = s.i[6] << s.i[4];
-    const long long want = wgs > 0 ? 2 * cus / wgs : 1, most = keys / (4 * (s.i[0] == LBR_CACHE_F32 ? 32 : 64));
-    return (int)(want < most ? (want > 1 ? want : 1) : (most > 1 ? most : 1));
+    const long long wgs = paged_row_tiles(s) * s.i[1] * s.i[2], tile = s.i[0] == LBR_CACHE_F32 ? 32 : 64;
+    if (wgs <= 0) return 1;
+    const long long tiles = (s.i[6] << s.i[4]) / tile;
+    const long long two = std::min(2 * cus / wgs, tiles / 2), one = std::min(cus / wgs, tiles);
+    return (int)std::max(1LL, std::max(two, one));
 }
 
 size_t paged_tiles_workspace(const Step& s) {
