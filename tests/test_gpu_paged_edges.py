@@ -8,11 +8,11 @@ import pytest
 import torch   # before the library's first use, so that both take the same HIP runtime
 
 from helpers import rng
-from paged_reference import Pages
+from paged_reference import Pages, verify
 from runtime.ir import Graph, OpType
 from runtime.paged import CACHE_TYPES, CacheLayout
 from runtime.session import Session
-from test_gpu_paged import TABLE, Ops, rows, step_session, tables
+from test_gpu_paged import TABLE, Ops, rows, run_verify, step_session, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -247,3 +247,30 @@ def test_c_entry_points(hip_lib, entry, S):
     pages.write(k, v, *where)
     check(y, pages, q, *where)
     ex.close()
+
+
+@pytest.mark.parametrize("B,S,T", [(2, 0, 3), (2, 1, 0), (0, 3, 3), (0, 0, 0)])
+def test_sizes_of_zero(B, S, T):
+    r = rng(1)
+    lay = CacheLayout(2, 64, 16, "int8")
+    pages = Pages.random(lay, 9, r)
+    where = (tables(r, B, 4, 9), np.full(B, 5, np.int32), np.full(B, S, np.int32))
+    q, k, v = (np.zeros((B, h, S, 64), np.float32) for h in (4, 2, 2))
+    ops = Ops(lay, pages)
+    ops.write(k, v, *where)
+    ops.attention(q, *where)
+    ops.read(T, *where)
+    out, after = ops.run()
+    pages.write(k, v, *where)
+    assert out["y"].shape == (B, 4, S, 64)
+    np.testing.assert_array_equal(out["z"], pages.read(*where, T).astype(np.float32))
+    np.testing.assert_array_equal(after, pages.pack())
+
+
+@pytest.mark.parametrize("B,D", [(0, 3), (2, 0), (0, 0)])
+def test_verify_of_nothing(B, D):
+    r = rng(2)
+    p = r.dirichlet(np.ones(7), (B, D + 1)).astype(np.float32).reshape(B, D + 1, 7)
+    ins = (p, np.zeros((B, D, 7), np.float32), np.zeros((B, D), np.int64), r.random((B, D + 1), dtype=np.float32),
+           np.zeros(B, np.int32))
+    np.testing.assert_array_equal(run_verify(*ins), verify(*ins))

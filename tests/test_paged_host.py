@@ -336,3 +336,27 @@ def test_graph_file_keeps_what_a_state_holds_at_first(tmp_path):
     g.tensors["cache"].buffer = r.integers(0, 256, g.tensors["cache"].shape, dtype=np.uint8)
     g.save(tmp_path / "g")
     np.testing.assert_array_equal(Graph.load(tmp_path / "g").tensors["cache"].buffer, g.tensors["cache"].buffer)
+
+
+class OnDevice:
+    """What a tensor in device memory shows of itself."""
+
+    def __init__(self, shape=(4, 6), typestr="<f4", at=1 << 20, strides=None, index=0):
+        self.__cuda_array_interface__ = {"shape": shape, "typestr": typestr, "data": (at, False), "strides": strides,
+                                         "version": 2}
+        self.device = type("Device", (), {"index": index})()
+
+
+def test_device_tensors_are_checked_against_the_graph():
+    from runtime.executor.compiled import _device_range
+
+    def address(t):
+        return _device_range(t, "q", (4, 6), "float32", 0)
+
+    assert address(OnDevice()) == address(OnDevice(strides=(24, 4))) == 1 << 20
+    for bad, error in ((np.zeros((4, 6), np.float32), "not in device memory"), (OnDevice(index=1), "on device 1"),
+                       (OnDevice(shape=(6, 4)), "shape"), (OnDevice(typestr="<f8"), "float64"),
+                       (OnDevice(strides=(4, 16)), "contiguous"), (OnDevice(strides=(48, 4)), "contiguous"),
+                       (OnDevice(at=(1 << 20) + 4), "16-byte")):
+        with pytest.raises((TypeError, ValueError), match=error):
+            address(bad)
