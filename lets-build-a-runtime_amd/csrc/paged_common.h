@@ -47,11 +47,11 @@ __device__ __forceinline__ char* cache_head(const PagedCache& c, int b, int h, l
 // Max over the aligned groups of G lanes that hold a row.
 template <int G>
 __device__ __forceinline__ unsigned row_max_bits(unsigned v) {
-    static_assert(G == 16 || G == 32 || G == 64, "lanes of a row");
+    static_assert(G == 8 || G == 16 || G == 32 || G == 64, "lanes of a row");
     v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false));
     v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, false));
     v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, false));
-    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, false));
+    if (G >= 16) v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, false));
     if (G >= 32) {
         auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
         v = max((unsigned)a[0], (unsigned)a[1]);
