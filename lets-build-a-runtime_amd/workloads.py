@@ -275,6 +275,8 @@ class Generator:
 
     def __init__(self, model: CachedLM, batch: int, draft: CachedLM | None = None, drafts: int = 3) -> None:
         lay = model.h[0].layout
+        if batch < 1 or drafts < 1:
+            raise ValueError(f"{batch} sequences of {drafts} drafted tokens")
         self.batch, self.drafts = batch, drafts if draft is not None else 0
         self.wide = model.h[0].cache.shape[0] // batch
         if self.wide < 1:

@@ -297,6 +297,9 @@ def test_generator_refusals(monkeypatch):
     m = language_model(1)
     with pytest.raises(ValueError, match="too small"):
         wl.Generator(m, 19)
+    for batch, drafts in ((0, 3), (3, 0)):
+        with pytest.raises(ValueError, match="drafted tokens"):
+            wl.Generator(m, batch, drafts=drafts)
     with pytest.raises(ValueError, match="drafting model"):
         wl.Generator(m, 3, draft=language_model(1, pages=17))
     gen = wl.Generator(m, 3)
